@@ -16,6 +16,11 @@ from torch.utils.cpp_extension import BuildExtension, CUDAExtension  # noqa: E40
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "gradient_accumulation_tf_estimator_amd", "ops", "csrc")
 
+# hipcc -O3 turns ordinary float code into the packed FP32 forms
+# (v_pk_add/mul/fma_f32); they are kept out of every kernel. The host pass
+# does not know the feature and only warns.
+NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+
 setup(
     name="gradient_accumulation_tf_estimator_amd",
     version="0.1.0",
@@ -49,7 +54,7 @@ setup(
             extra_compile_args={
                 "cxx": ["-O3"] + (["-fsanitize=address", "-g"]
                                   if os.environ.get("GA_ASAN") else []),
-                "nvcc": ["-O3", "--offload-arch=gfx950"]
+                "nvcc": ["-O3", "--offload-arch=gfx950"] + NO_PACKED_FP32
                 + (["-fsanitize=address", "-g",
                     "-Xarch_device", "-fno-sanitize=all"]
                    if os.environ.get("GA_ASAN") else []),

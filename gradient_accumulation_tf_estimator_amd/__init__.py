@@ -10,6 +10,7 @@ from .engine.optimizer import TrainOp, create_optimizer
 from .engine.accum import AccumEngine
 from .engine.schedule import learning_rate
 from .engine.flat import DEFAULT_EXCLUDE_FROM_WEIGHT_DECAY
+from .ops.clip import clip_by_global_norm, global_norm
 
 __version__ = "0.1.0"
 
@@ -19,4 +20,6 @@ __all__ = [
     "AccumEngine",
     "learning_rate",
     "DEFAULT_EXCLUDE_FROM_WEIGHT_DECAY",
+    "clip_by_global_norm",
+    "global_norm",
 ]

@@ -1,0 +1,78 @@
+"""Global norm over many tensors, and clipping by it.
+
+The engine clips its own flat fp32 buffer inside the apply kernel. These two
+are for gradients that live in tensors of their own: any number, of any shape,
+bf16, fp16 and fp32 in one list. Semantics are ``tf.clip_by_global_norm``'s,
+which the reference calls on its list of gradients (optimization.py:84):
+
+    norm = sqrt(sum_i sum(t_i^2));  out_i = t_i * clip_norm / max(norm, clip_norm)
+
+and where the norm is infinite or NaN every output is NaN. ``None`` entries are
+passed through. Sums are held in 64 bits. Nothing waits for the GPU: the norm
+stays on the device, and a call can be captured into a graph (which then holds
+the tensors' addresses).
+"""
+
+from __future__ import annotations
+
+import math
+from typing import List, Optional, Sequence, Tuple
+
+import torch
+
+from . import require_hip
+
+Tensors = Sequence[Optional[torch.Tensor]]
+
+
+def _present(tensors: Tensors) -> List[torch.Tensor]:
+    if isinstance(tensors, torch.Tensor):
+        raise TypeError("expected a list of tensors")
+    got = [t.detach() for t in tensors if t is not None]
+    for t in got:
+        if t.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+            raise ValueError(f"tensors must be fp32, bf16 or fp16, got {t.dtype}")
+        if t.device != got[0].device:
+            raise ValueError("tensors must be on one device")
+    return got
+
+
+def global_norm(tensors: Tensors) -> torch.Tensor:
+    """2-norm of all elements of all tensors, an fp32 scalar on their device."""
+    got = _present(tensors)
+    if not got:
+        return torch.zeros(())
+    if got[0].is_cuda:
+        return require_hip().global_norm(got, [], 1.0)
+    return torch.stack([t.double().square().sum() for t in got]).sum().sqrt().float()
+
+
+def clip_by_global_norm(tensors: Tensors, clip_norm: float, *,
+                        out: Optional[Tensors] = None) -> Tuple[List[Optional[torch.Tensor]], torch.Tensor]:
+    """-> (clipped tensors, norm before clipping). ``out`` takes the results:
+    tensors like the inputs (same dtype, shape and strides), or the inputs
+    themselves to clip in place; an output may share memory with its own input
+    alone. Without it new tensors are returned."""
+    if not (clip_norm > 0):
+        raise ValueError(f"clip_norm must be positive, got {clip_norm}")
+    got = _present(tensors)
+    if out is None:
+        new = [None if t is None else torch.empty_like(t, requires_grad=False) for t in tensors]
+    else:
+        new = list(out)
+        if len(new) != len(tensors) or any((a is None) != (b is None) for a, b in zip(new, tensors)):
+            raise ValueError("out must have an entry for each tensor, and None where it has None")
+    if not got:
+        return new, torch.zeros(())
+    dst = [t.detach() for t in new if t is not None]
+    if got[0].is_cuda:
+        return new, require_hip().global_norm(got, dst, float(clip_norm))
+    norm = torch.stack([t.double().square().sum() for t in got]).sum().sqrt()
+    n = float(norm)
+    coef = math.nan if not math.isfinite(n) else 1.0 if n <= clip_norm else clip_norm / n
+    coef = torch.tensor(coef, dtype=torch.float32)
+    for d, t in zip(dst, got):
+        if d.shape != t.shape or d.dtype != t.dtype or d.device != t.device:
+            raise ValueError("an output must have its tensor's device, dtype and shape")
+        d.copy_(t.float() * coef)
+    return new, norm.float()

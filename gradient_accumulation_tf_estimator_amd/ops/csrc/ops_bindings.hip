@@ -1,0 +1,246 @@
+// PyTorch bindings of the norm, clipping and relative-attention kernels: checks
+// of shapes, types and alignment, allocation of outputs, launches on the
+// current stream of the operands' device.
+
+#include <algorithm>
+#include <cstdint>
+#include <vector>
+
+#include <ATen/hip/HIPContext.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
+#include <torch/extension.h>
+
+#include "ga_ops.h"
+
+namespace {
+
+typedef c10::optional<at::Tensor> MaybeTensor;
+
+int type_of(const at::Tensor& t, const char* name) {
+  switch (t.scalar_type()) {
+    case at::kFloat: return GA_FP32;
+    case at::kBFloat16: return GA_BF16;
+    case at::kHalf: return GA_FP16;
+    default: TORCH_CHECK(false, name, " must be fp32, bf16 or fp16, got ", t.scalar_type());
+  }
+}
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+hipStream_t stream_of(const at::Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
+
+void check_launch(hipError_t e, const char* what) {
+  TORCH_CHECK(e == hipSuccess, what, " launch failed: ", hipGetErrorString(e));
+}
+
+// ---------------- root-mean-square norm ----------------
+
+const int kMaxNormWidth = 8192;
+
+// rows [R, H] with neighbouring columns and any row stride; whether 16-byte
+// accesses may be used
+bool check_rows(const at::Tensor& t, const char* name, const at::Tensor& like) {
+  TORCH_CHECK(t.is_cuda() && t.device() == like.device(), name, " must be on the GPU that holds x");
+  TORCH_CHECK(t.scalar_type() == like.scalar_type(), name, " must have x's dtype");
+  TORCH_CHECK(t.dim() == 2 && t.size(0) == like.size(0) && t.size(1) == like.size(1),
+              name, " must be [rows, hidden] like x");
+  TORCH_CHECK(t.numel() == 0 || t.size(1) == 1 || t.stride(1) == 1, name, "'s columns must be contiguous");
+  return aligned16(t.data_ptr()) && (t.size(0) <= 1 || t.stride(0) % 8 == 0);
+}
+
+RmsArgs norm_args(const at::Tensor& x, const at::Tensor& w, double eps, bool& vec) {
+  TORCH_CHECK(x.dim() == 2, "x must be [rows, hidden]");
+  type_of(x, "x");
+  const int64_t H = x.size(1);
+  TORCH_CHECK(H >= 1 && H <= kMaxNormWidth, "RMS norm width must be 1..", kMaxNormWidth, ", got ", H);
+  vec = check_rows(x, "x", x) && H % 8 == 0;
+  TORCH_CHECK(w.is_cuda() && w.device() == x.device() && w.scalar_type() == x.scalar_type() &&
+              w.dim() == 1 && w.numel() == H && w.is_contiguous(),
+              "weight must be a contiguous [hidden] tensor of x's dtype and device");
+  vec = vec && aligned16(w.data_ptr());
+  TORCH_CHECK(eps >= 0, "eps must not be negative");
+  RmsArgs a = {};
+  a.x = x.data_ptr();
+  a.x_stride = x.stride(0);
+  a.w = w.data_ptr();
+  a.R = x.size(0);
+  a.H = (int)H;
+  a.eps = (float)eps;
+  return a;
+}
+
+std::vector<at::Tensor> rms_norm_fwd(at::Tensor x, MaybeTensor res, at::Tensor w, double eps) {
+  bool vec;
+  RmsArgs a = norm_args(x, w, eps, vec);
+  const c10::OptionalDeviceGuard guard(x.device());
+  auto y = at::empty({x.size(0), x.size(1)}, x.options());
+  auto h = res ? at::empty({x.size(0), x.size(1)}, x.options()) : x;
+  auto rstd = at::empty({x.size(0)}, x.options().dtype(at::kFloat));
+  if (res) {
+    vec = check_rows(*res, "residual", x) && vec;
+    a.res = res->data_ptr();
+    a.res_stride = res->stride(0);
+    a.h = h.data_ptr();
+  }
+  if (a.R == 0) return {y, h, rstd};
+  a.y = y.data_ptr();
+  a.rstd = rstd.data_ptr<float>();
+  check_launch(rms_forward(type_of(x, "x"), vec, a, stream_of(x)), "rms_norm_fwd");
+  return {y, h, rstd};
+}
+
+// dw_acc: an fp32 slice that dw is added to; the second result is then empty
+std::vector<at::Tensor> rms_norm_bwd(at::Tensor dy, MaybeTensor dh, at::Tensor h, at::Tensor w,
+                                     at::Tensor rstd, MaybeTensor dw_acc) {
+  bool vec;
+  RmsArgs a = norm_args(h, w, 0.0, vec);
+  const c10::OptionalDeviceGuard guard(h.device());
+  vec = check_rows(dy, "dy", h) && vec;
+  TORCH_CHECK(rstd.device() == h.device() && rstd.scalar_type() == at::kFloat && rstd.is_contiguous() &&
+              rstd.numel() == h.size(0), "rstd must be the forward's");
+  if (dh) {
+    vec = check_rows(*dh, "dh", h) && vec;
+    a.dh = dh->data_ptr();
+    a.dh_stride = dh->stride(0);
+  }
+  if (dw_acc)
+    TORCH_CHECK(dw_acc->device() == h.device() && dw_acc->scalar_type() == at::kFloat &&
+                dw_acc->is_contiguous() && dw_acc->numel() == a.H, "dw_acc must be an fp32 [hidden] slice");
+  auto dx = at::empty({h.size(0), h.size(1)}, h.options());
+  auto dw = dw_acc ? at::Tensor() : at::empty({a.H}, w.options());
+  if (a.R == 0) {
+    if (dw.defined()) dw.zero_();
+    return {dx, dw};
+  }
+  auto slabs = at::empty({rms_slabs(a.R, a.H), a.H}, h.options().dtype(at::kFloat));
+  a.dy = dy.data_ptr();
+  a.dy_stride = dy.stride(0);
+  a.rstd = rstd.data_ptr<float>();
+  a.y = dx.data_ptr();
+  a.slabs = slabs.data_ptr<float>();
+  check_launch(rms_backward(type_of(h, "h"), vec, a, dw.defined() ? dw.data_ptr() : nullptr,
+                            dw_acc ? dw_acc->data_ptr<float>() : nullptr, stream_of(h)), "rms_norm_bwd");
+  return {dx, dw};
+}
+
+std::vector<at::Tensor> rms_norm_fp8(at::Tensor x, MaybeTensor res, at::Tensor w, double eps, int64_t group) {
+  bool vec;
+  RmsArgs a = norm_args(x, w, eps, vec);
+  const c10::OptionalDeviceGuard guard(x.device());
+  TORCH_CHECK(group == 0 || group == 32 || group == 64 || group == 128, "group must be 0 (a row), 32, 64 or 128");
+  TORCH_CHECK(group == 0 || a.H % group == 0, "hidden must be a multiple of the group");
+  const int64_t groups = group ? a.H / group : 1;
+  auto q = at::empty({x.size(0), x.size(1)}, x.options().dtype(at::kFloat8_e4m3fn));
+  auto scales = at::empty({x.size(0), groups}, x.options().dtype(at::kFloat));
+  auto h = res ? at::empty({x.size(0), x.size(1)}, x.options()) : x;
+  if (res) {
+    vec = check_rows(*res, "residual", x) && vec;
+    a.res = res->data_ptr();
+    a.res_stride = res->stride(0);
+    a.h = h.data_ptr();
+  }
+  if (a.R == 0) return {q, scales, h};
+  a.q = (unsigned char*)q.data_ptr();
+  a.scales = scales.data_ptr<float>();
+  a.group = (int)group;
+  check_launch(rms_fp8(type_of(x, "x"), vec, a, stream_of(x)), "rms_norm_fp8");
+  return {q, scales, h};
+}
+
+// ---------------- global norm and clipping ----------------
+
+// No output may lie over another output or over another tensor's input: the
+// blocks that read and write them run in no order. out[i] == in[i] is in place.
+void check_apart(const std::vector<at::Tensor>& ins, const std::vector<at::Tensor>& outs) {
+  struct Span { uintptr_t lo, hi; bool out; };
+  std::vector<Span> spans;
+  for (size_t i = 0; i < ins.size(); ++i) {
+    if (ins[i].numel() == 0) continue;
+    const uintptr_t a = (uintptr_t)ins[i].data_ptr(), b = (uintptr_t)outs[i].data_ptr();
+    spans.push_back({b, b + outs[i].nbytes(), true});
+    if (a != b) spans.push_back({a, a + ins[i].nbytes(), false});
+  }
+  std::sort(spans.begin(), spans.end(), [](const Span& x, const Span& y) { return x.lo < y.lo; });
+  uintptr_t out_end = 0, any_end = 0;
+  for (const Span& s : spans) {
+    TORCH_CHECK(s.lo >= (s.out ? any_end : out_end),
+                "an output shares memory with another tensor of the list (is one listed twice?)");
+    any_end = std::max(any_end, s.hi);
+    if (s.out) out_end = std::max(out_end, s.hi);
+  }
+}
+
+// Norm of all tensors; with `outs`, outs[i] = ins[i] * min(1, clip / norm).
+// Tensors are taken as their memory, whatever the order of their dimensions;
+// an output has to have its input's strides.
+at::Tensor global_norm(std::vector<at::Tensor> ins, std::vector<at::Tensor> outs, double clip) {
+  TORCH_CHECK(!ins.empty(), "global_norm needs at least one tensor");
+  const bool write = !outs.empty();
+  TORCH_CHECK(!write || outs.size() == ins.size(), "one output for each tensor");
+  TORCH_CHECK(!write || clip > 0, "clip_norm must be positive");
+  const auto dev = ins[0].device();
+  TORCH_CHECK(ins[0].is_cuda(), "tensors must be on a GPU");
+  const c10::OptionalDeviceGuard guard(dev);
+  long long total = 0;
+  for (size_t i = 0; i < ins.size(); ++i) {
+    TORCH_CHECK(ins[i].device() == dev, "tensors must be on one device");
+    type_of(ins[i], "tensor");
+    TORCH_CHECK(ins[i].is_non_overlapping_and_dense(), "tensor ", i,
+                " has gaps or overlaps in memory: pass a contiguous copy");
+    if (write)
+      TORCH_CHECK(outs[i].device() == dev && outs[i].scalar_type() == ins[i].scalar_type() &&
+                  outs[i].sizes() == ins[i].sizes() && outs[i].strides() == ins[i].strides(),
+                  "output ", i, " must have its tensor's device, dtype, shape and strides");
+    total += ins[i].numel();
+  }
+  if (write) check_apart(ins, outs);
+  // about 4096 blocks for large sets, at least 8192 elements a block
+  long long chunk = (total / 4096 + 2047) / 2048 * 2048;
+  if (chunk < 8192) chunk = 8192;
+  TORCH_CHECK(chunk <= (1ll << 30), "too many elements");
+  std::vector<ClipArgs> launches;
+  long long blocks = 0;
+  for (size_t i = 0; i < ins.size(); ++i) {
+    const long long n = ins[i].numel();
+    if (n == 0) continue;
+    if (launches.empty() || launches.back().count == GA_CLIP_TENSORS) {
+      launches.emplace_back();
+      launches.back().count = 0;
+      launches.back().first[0] = 0;
+      launches.back().chunk = (int)chunk;
+    }
+    ClipArgs& a = launches.back();
+    const int t = a.count++;
+    a.in[t] = ins[i].data_ptr();
+    a.out[t] = write ? outs[i].data_ptr() : nullptr;
+    a.n[t] = n;
+    a.type[t] = (unsigned char)type_of(ins[i], "tensor");
+    a.vec[t] = aligned16(a.in[t]) && aligned16(a.out[t]);
+    a.first[t + 1] = a.first[t] + (int)((n + chunk - 1) / chunk);
+    blocks += (n + chunk - 1) / chunk;
+  }
+  auto sums = at::empty({blocks}, ins[0].options().dtype(at::kDouble));
+  auto result = at::empty({2}, ins[0].options().dtype(at::kFloat));  // norm, factor
+  hipStream_t s = stream_of(ins[0]);
+  long long at_block = 0;
+  for (const auto& a : launches) {
+    check_launch(clip_sums(a, sums.data_ptr<double>() + at_block, s), "global_norm");
+    at_block += a.first[a.count];
+  }
+  float* r = result.data_ptr<float>();
+  check_launch(clip_finish(blocks ? sums.data_ptr<double>() : nullptr, (int)blocks, clip, r, write ? r + 1 : nullptr, s),
+               "global_norm");
+  if (write)
+    for (const auto& a : launches) check_launch(clip_scale(a, r + 1, s), "clip_by_global_norm");
+  return result.select(0, 0);
+}
+
+}  // namespace
+
+void register_ops(pybind11::module_& mod) {
+  mod.def("rms_norm_fwd", &rms_norm_fwd, "x (+ residual) -> y, h, rstd");
+  mod.def("rms_norm_bwd", &rms_norm_bwd, "dy (+ dh) -> dx, dw (or dw added to an fp32 slice)");
+  mod.def("rms_norm_fp8", &rms_norm_fp8, "x (+ residual) -> e4m3 values, scales, h");
+  mod.def("global_norm", &global_norm, "norm over many tensors; with outputs, clipped copies");
+}

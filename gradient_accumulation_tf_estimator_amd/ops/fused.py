@@ -738,6 +738,7 @@ def direct_param_names(model: nn.Module):
     passed to FlatState so K1 can skip their (contiguous) flat region."""
     names = []
     by_mod = {id(m): n for n, m in model.named_modules()}
+    from .rms_norm import FusedAddRMSNorm
 
     def pname(mod, attr):
         prefix = by_mod[id(mod)]
@@ -749,6 +750,8 @@ def direct_param_names(model: nn.Module):
             names.append(pname(mod, "bias"))
             if mod.proj_bias is not None:
                 names.append(pname(mod, "proj_bias"))
+        elif isinstance(mod, FusedAddRMSNorm):
+            names.append(pname(mod, "weight"))
         elif isinstance(mod, FusedBiasGelu):
             names.append(pname(mod, "bias"))
         elif isinstance(mod, (DirectLinear, DirectEmbedding)):
@@ -770,9 +773,14 @@ def bind_direct_grad(model: nn.Module, engine) -> int:
     slices. Returns the number of modules bound. No-op for non-hip engines."""
     if engine.backend != "hip":
         return 0
+    from .rms_norm import FusedAddRMSNorm
+
     n = 0
     for mod in model.modules():
-        if isinstance(mod, FusedAddLayerNorm):
+        if isinstance(mod, FusedAddRMSNorm):
+            mod._accum_view = engine.state.accum_view(mod.weight)
+            n += 1
+        elif isinstance(mod, FusedAddLayerNorm):
             mod._accum_views = (
                 engine.state.accum_view(mod.weight),
                 engine.state.accum_view(mod.bias),

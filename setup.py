@@ -39,6 +39,9 @@ setup(
                 os.path.join(CSRC, "ffn_mfma.hip"),
                 os.path.join(CSRC, "cls_head.hip"),
                 os.path.join(CSRC, "linear_small.hip"),
+                os.path.join(CSRC, "rms_norm.hip"),
+                os.path.join(CSRC, "grad_clip.hip"),
+                os.path.join(CSRC, "ops_bindings.hip"),
                 os.path.join(CSRC, "ga_bindings.hip"),
             ],
             libraries=["hipblaslt"],

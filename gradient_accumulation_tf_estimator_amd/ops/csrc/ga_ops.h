@@ -43,3 +43,42 @@ struct ClipArgs {
 hipError_t clip_sums(const ClipArgs& a, double* sums, hipStream_t s);
 hipError_t clip_finish(const double* sums, int n, double clip, float* norm, float* coef, hipStream_t s);
 hipError_t clip_scale(const ClipArgs& a, const float* coef, hipStream_t s);
+
+// ---- attention with a relative position bias (rel_attn.hip); strides in elements ----
+#define GA_REL_MAX_DISTANCE 1024
+#define GA_REL_MAX_BUCKETS 256
+struct RelArgs {
+  const __bf16 *q, *k, *v;
+  long long q_b, q_s, q_h, k_b, k_s, k_h, v_b, v_s, v_h;
+  const __bf16* table;        // [buckets][NH]
+  const int* map;             // [2 * far + 1], the bucket of each offset
+  const unsigned char* mask;  // [B][S], 1 = attend, or null
+  __bf16* out;                // [B][S][NH][D]
+  float* lse;                 // [B][NH][S], base 2; +inf for a row with nothing allowed
+  // backward
+  const __bf16* dout;         // [B][S][NH][D]
+  float* dsum;                // [B][NH][S]
+  __bf16 *dq, *dk, *dv;       // strides of q, k and v below
+  long long dq_b, dq_s, dk_b, dk_s;  // heads lie D apart
+  float* doff;                // [B * NH * tiles][2 * far + 1], tiles = rel_tiles(S)
+  __bf16* dtable;             // [buckets][NH]
+  int B, S, NH, NKV, D, buckets, far, causal;
+  float scale;
+};
+int rel_tiles(int S);
+hipError_t rel_forward(const RelArgs& a, hipStream_t s);
+hipError_t rel_backward(const RelArgs& a, hipStream_t s);
+
+struct RelTokenArgs {
+  const __bf16 *q, *k, *v;
+  long long q_b, q_s, q_h, k_b, k_s, k_h, v_b, v_s, v_h;
+  const __bf16* table;
+  const int* map;
+  const int* lengths;  // [B]
+  __bf16* out;         // [B][Sq][NH][D]
+  float* parts;        // [B * NKV * row tiles][splits][32][D + 2]
+  int B, Sq, S, NH, NKV, D, buckets, far, splits;
+  float scale;
+};
+int rel_token_splits(int B, int Sq, int S, int NH, int NKV);
+hipError_t rel_token(const RelTokenArgs& a, hipStream_t s);

@@ -3,6 +3,7 @@
 // current stream of the operands' device.
 
 #include <algorithm>
+#include <cmath>
 #include <cstdint>
 #include <vector>
 
@@ -236,11 +237,164 @@ at::Tensor global_norm(std::vector<at::Tensor> ins, std::vector<at::Tensor> outs
   return result.select(0, 0);
 }
 
+// ---------------- attention with a relative position bias ----------------
+
+void check_bias(const at::Tensor& table, const at::Tensor& map, const at::Tensor& like, int64_t NH) {
+  TORCH_CHECK(table.device() == like.device() && table.scalar_type() == at::kBFloat16 && table.is_contiguous() &&
+              table.dim() == 2 && table.size(1) == NH, "the bias table must be a contiguous bf16 [buckets, heads] tensor");
+  TORCH_CHECK(table.size(0) >= 1 && table.size(0) <= GA_REL_MAX_BUCKETS, "buckets must be 1..", GA_REL_MAX_BUCKETS);
+  TORCH_CHECK(map.device() == like.device() && map.scalar_type() == at::kInt && map.is_contiguous() && map.dim() == 1 &&
+              map.numel() % 2 == 1 && map.numel() >= 3 && map.numel() <= 2 * GA_REL_MAX_DISTANCE + 1,
+              "the bucket map must be an int32 [2 * max_distance + 1] tensor, max_distance 1..", GA_REL_MAX_DISTANCE);
+}
+
+void check_heads(int64_t NH, int64_t NKV, int64_t D) {
+  TORCH_CHECK(D == 64 || D == 128, "head size must be 64 or 128, got ", D);
+  TORCH_CHECK(NH >= 1 && NKV >= 1 && NH % NKV == 0, "query heads must be a multiple of key/value heads");
+}
+
+RelArgs rel_args(const at::Tensor& qkv, int64_t NH, int64_t NKV, const at::Tensor& table, const at::Tensor& map,
+                 const MaybeTensor& mask, bool causal, double scale) {
+  TORCH_CHECK(qkv.is_cuda() && qkv.scalar_type() == at::kBFloat16 && qkv.dim() == 3 && qkv.is_contiguous() &&
+              aligned16(qkv.data_ptr()), "qkv must be a contiguous, 16-byte aligned bf16 [B, S, (NH + 2 NKV) D] GPU tensor");
+  TORCH_CHECK(NH >= 1 && NKV >= 1 && qkv.size(2) % (NH + 2 * NKV) == 0, "qkv's last dimension must be (NH + 2 NKV) * D");
+  const int64_t B = qkv.size(0), S = qkv.size(1), D = qkv.size(2) / (NH + 2 * NKV);
+  check_heads(NH, NKV, D);
+  check_bias(table, map, qkv, NH);
+  TORCH_CHECK(scale > 0 && std::isfinite(scale), "scale must be positive and finite");
+  TORCH_CHECK(S < (1ll << 24) && B * NH * (S / 128 + 1) < (1ll << 31), "too many rows");
+  if (mask)
+    TORCH_CHECK(mask->device() == qkv.device() && mask->scalar_type() == at::kByte && mask->is_contiguous() &&
+                mask->dim() == 2 && mask->size(0) == B && mask->size(1) == S, "mask must be a contiguous u8 [B, S] tensor");
+  RelArgs a = {};
+  const __bf16* p = (const __bf16*)qkv.data_ptr();
+  a.q = p;
+  a.k = p + NH * D;
+  a.v = p + (NH + NKV) * D;
+  a.q_b = a.k_b = a.v_b = S * qkv.size(2);
+  a.q_s = a.k_s = a.v_s = qkv.size(2);
+  a.q_h = a.k_h = a.v_h = D;
+  a.table = (const __bf16*)table.data_ptr();
+  a.map = map.data_ptr<int>();
+  a.mask = mask ? mask->data_ptr<unsigned char>() : nullptr;
+  a.B = (int)B;
+  a.S = (int)S;
+  a.NH = (int)NH;
+  a.NKV = (int)NKV;
+  a.D = (int)D;
+  a.buckets = (int)table.size(0);
+  a.far = (int)(map.numel() / 2);
+  a.causal = causal;
+  a.scale = (float)scale;
+  return a;
+}
+
+// -> out [B, S, NH * D], lse [B, NH, S] (empty unless wanted)
+std::vector<at::Tensor> rel_attn_fwd(at::Tensor qkv, int64_t NH, int64_t NKV, at::Tensor table, at::Tensor map,
+                                     MaybeTensor mask, bool causal, double scale, bool want_lse) {
+  RelArgs a = rel_args(qkv, NH, NKV, table, map, mask, causal, scale);
+  const c10::OptionalDeviceGuard guard(qkv.device());
+  auto out = at::empty({a.B, a.S, NH * a.D}, qkv.options());
+  auto lse = want_lse ? at::empty({a.B, NH, a.S}, qkv.options().dtype(at::kFloat)) : at::Tensor();
+  if (out.numel() == 0) return {out, lse};
+  a.out = (__bf16*)out.data_ptr();
+  a.lse = want_lse ? lse.data_ptr<float>() : nullptr;
+  check_launch(rel_forward(a, stream_of(qkv)), "rel_attn_fwd");
+  return {out, lse};
+}
+
+// -> dqkv like qkv, dtable like table
+std::vector<at::Tensor> rel_attn_bwd(at::Tensor dout, at::Tensor qkv, at::Tensor out, at::Tensor lse, int64_t NH,
+                                     int64_t NKV, at::Tensor table, at::Tensor map, MaybeTensor mask, bool causal,
+                                     double scale) {
+  RelArgs a = rel_args(qkv, NH, NKV, table, map, mask, causal, scale);
+  const c10::OptionalDeviceGuard guard(qkv.device());
+  for (const auto& t : {dout, out})
+    TORCH_CHECK(t.device() == qkv.device() && t.scalar_type() == at::kBFloat16 && t.is_contiguous() &&
+                t.numel() == (int64_t)a.B * a.S * NH * a.D && aligned16(t.data_ptr()),
+                "dout and out must be contiguous, 16-byte aligned bf16 [B, S, NH * D] tensors");
+  TORCH_CHECK(lse.device() == qkv.device() && lse.scalar_type() == at::kFloat && lse.is_contiguous() &&
+              lse.numel() == (int64_t)a.B * NH * a.S, "lse must be the forward's");
+  auto dqkv = at::empty_like(qkv);
+  auto dtable = at::empty_like(table);
+  if (dqkv.numel() == 0) {
+    dtable.zero_();
+    return {dqkv, dtable};
+  }
+  auto dsum = at::empty_like(lse);
+  auto doff = at::empty({(int64_t)a.B * NH * rel_tiles(a.S), 2 * a.far + 1}, lse.options());
+  a.out = (__bf16*)out.data_ptr();
+  a.lse = lse.data_ptr<float>();
+  a.dout = (const __bf16*)dout.data_ptr();
+  a.dsum = dsum.data_ptr<float>();
+  a.doff = doff.data_ptr<float>();
+  a.dtable = (__bf16*)dtable.data_ptr();
+  a.dq = (__bf16*)dqkv.data_ptr();
+  a.dk = a.dq + NH * a.D;
+  a.dv = a.dk + NKV * a.D;
+  a.dq_b = a.dk_b = a.q_b;
+  a.dq_s = a.dk_s = a.q_s;
+  check_launch(rel_backward(a, stream_of(qkv)), "rel_attn_bwd");
+  return {dqkv, dtable};
+}
+
+// q [B, Sq, NH, D], caches [B, S, NKV, D] of any strides with contiguous, 16-byte aligned rows
+at::Tensor rel_attn_token(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor table, at::Tensor map,
+                          at::Tensor lengths, double scale) {
+  TORCH_CHECK(q.is_cuda() && q.dim() == 4 && k.dim() == 4 && v.dim() == 4, "q, k and v must be 4-dimensional GPU tensors");
+  const int64_t B = q.size(0), Sq = q.size(1), NH = q.size(2), D = q.size(3), S = k.size(1), NKV = k.size(2);
+  check_heads(NH, NKV, D);
+  TORCH_CHECK(k.sizes() == v.sizes() && k.size(0) == B && k.size(3) == D, "caches must be [B, S, NKV, D] with q's B and D");
+  for (const auto& t : {q, k, v}) {
+    TORCH_CHECK(t.device() == q.device() && t.scalar_type() == at::kBFloat16, "q, k and v must be bf16 on one GPU");
+    TORCH_CHECK(t.numel() == 0 || (t.stride(3) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 &&
+                t.stride(2) % 8 == 0 && aligned16(t.data_ptr())),
+                "q, k and v need contiguous heads that start on 16 bytes");
+  }
+  check_bias(table, map, q, NH);
+  TORCH_CHECK(lengths.device() == q.device() && lengths.scalar_type() == at::kInt && lengths.is_contiguous() &&
+              lengths.dim() == 1 && lengths.numel() == B, "lengths must be an int32 [B] tensor on the same GPU");
+  TORCH_CHECK(scale > 0 && std::isfinite(scale), "scale must be positive and finite");
+  TORCH_CHECK(NH / NKV <= 32, "at most 32 query heads a key/value head");
+  TORCH_CHECK(S < (1ll << 31) - 64 && B * NH * Sq < (1ll << 24), "too many rows");
+  const c10::OptionalDeviceGuard guard(q.device());
+  auto out = at::empty({B, Sq, NH, D}, q.options());
+  if (out.numel() == 0) return out;
+  if (S == 0) return out.zero_();
+  RelTokenArgs a = {};
+  a.q = (const __bf16*)q.data_ptr();
+  a.k = (const __bf16*)k.data_ptr();
+  a.v = (const __bf16*)v.data_ptr();
+  a.q_b = q.stride(0); a.q_s = q.stride(1); a.q_h = q.stride(2);
+  a.k_b = k.stride(0); a.k_s = k.stride(1); a.k_h = k.stride(2);
+  a.v_b = v.stride(0); a.v_s = v.stride(1); a.v_h = v.stride(2);
+  a.table = (const __bf16*)table.data_ptr();
+  a.map = map.data_ptr<int>();
+  a.lengths = lengths.data_ptr<int>();
+  a.out = (__bf16*)out.data_ptr();
+  a.B = (int)B; a.Sq = (int)Sq; a.S = (int)S; a.NH = (int)NH; a.NKV = (int)NKV; a.D = (int)D;
+  a.buckets = (int)table.size(0);
+  a.far = (int)(map.numel() / 2);
+  a.scale = (float)scale;
+  a.splits = rel_token_splits(a.B, a.Sq, a.S, a.NH, a.NKV);
+  at::Tensor parts;
+  if (a.splits > 1) {
+    const int64_t tiles = (NH / NKV * Sq + 31) / 32;
+    parts = at::empty({B * NKV * tiles * a.splits, 32, D + 2}, q.options().dtype(at::kFloat));
+    a.parts = parts.data_ptr<float>();
+  }
+  check_launch(rel_token(a, stream_of(q)), "rel_attn_token");
+  return out;
+}
+
 }  // namespace
 
 void register_ops(pybind11::module_& mod) {
   mod.def("rms_norm_fwd", &rms_norm_fwd, "x (+ residual) -> y, h, rstd");
   mod.def("rms_norm_bwd", &rms_norm_bwd, "dy (+ dh) -> dx, dw (or dw added to an fp32 slice)");
   mod.def("rms_norm_fp8", &rms_norm_fp8, "x (+ residual) -> e4m3 values, scales, h");
+  mod.def("rel_attn_fwd", &rel_attn_fwd, "packed qkv + bucket bias -> out, lse");
+  mod.def("rel_attn_bwd", &rel_attn_bwd, "-> packed dqkv, dtable");
+  mod.def("rel_attn_token", &rel_attn_token, "new tokens over a K/V cache with a bucket bias");
   mod.def("global_norm", &global_norm, "norm over many tensors; with outputs, clipped copies");
 }

@@ -1,0 +1,885 @@
+// Attention with a learned relative position bias (gfx950), head size 64 or 128.
+//
+//   s_ij = scale <q_i, k_j> + beta_h(j - i),  beta_h(d) = table[map[clamp(d)]][h]
+//   P = softmax_j(s) over the keys allowed by the key mask (and j <= i),
+//   O = P V; a row with no key allowed is zero.
+//   dV = P^T dO, dP = dO V^T, D_i = <dO_i, O_i>, dS = P (dP - D),
+//   dQ = scale dS K, dK = scale dS^T Q, dtable[n][h] = sum of dS where map = n
+//
+// Layout. v_mfma_f32_32x32x16_bf16: A[m][k] has m = lane & 31, k = 8 (lane >> 5)
+// + e; B[k][n] likewise; C has column lane & 31 and row (r & 3) + 8 (r >> 2) +
+// 4 (lane >> 5). Every product is written so that the axis that a softmax row
+// or a gradient row belongs to is the C column: a lane then owns a whole query
+// (or key), its maximum and sum are registers, and the one cross-lane step is
+// between the two halves of the wave. The second product contracts over C's
+// rows: its B operand is C itself, rounded, with the rows in the order that the
+// registers hold them, and its A operand is read from LDS in that same order by
+// the transposing 64-bit read (each lane gets four rows of one column). So no
+// tile is ever exchanged between lanes or written back.
+//
+// The bias enters as C's initial value (beta / scale), so it costs no addition:
+// where all of a 32x32 tile is further than the largest distance it is one
+// constant, else four neighbouring offsets come as one 16-byte LDS read from a
+// table kept in four copies, each shifted by one entry, so that every start is
+// aligned.
+//
+// 32 bits: scores, maxima, sums, D, dS for the table's gradient, accumulators.
+// Rounded to bf16: P and dS before the second product (a relative 2^-9 of each,
+// which the matrix instruction's operands force), and the outputs.
+
+#include <hip/hip_runtime.h>
+
+#include "ga_ops.h"
+
+namespace {
+
+typedef __attribute__((ext_vector_type(8))) __bf16 b8;
+typedef __attribute__((ext_vector_type(4))) __bf16 b4;
+typedef __attribute__((ext_vector_type(4))) short s4;
+typedef __attribute__((ext_vector_type(8))) short s8;
+typedef __attribute__((ext_vector_type(4))) float f4;
+typedef __attribute__((ext_vector_type(16))) float f16;
+typedef __attribute__((address_space(3))) s4 lds_s4;
+
+#define LOG2E 1.44269504088896340736f
+#define INF __builtin_inff()
+
+constexpr int KC = 64;     // rows of a staged chunk
+constexpr int TILE = 128;  // rows of a workgroup: four waves of 32
+
+// ---- LDS tiles: [rows][D] bf16, 16-byte pieces XORed by the row. Eight
+// neighbouring rows spread over the eight pieces of 128 bytes (the row reads of
+// 32 lanes), and four neighbouring rows over four pairs (the transposing
+// reads): both are free of bank conflicts.
+template <int D>
+__device__ __forceinline__ int piece(int row, int p) {
+  const int f = ((row & 3) << 1) | ((row >> 2) & 1);
+  return row * 2 * D + ((p ^ f) << 4);
+}
+
+// A fragment, rows of the tile as m: row `row`, columns 16 t + 8 hi ..
+template <int D>
+__device__ __forceinline__ b8 row_frag(const char* tile, int row, int t, int hi) {
+  return *(const b8*)(tile + piece<D>(row, 2 * t + hi));
+}
+
+// A fragment, columns of the tile as m (32 dt ..), 16 rows from `row` as k in
+// the order of C's registers
+template <int D>
+__device__ __forceinline__ b8 col_frag(const char* tile, int row, int dt, int lane) {
+  const int t = lane & 15, r = row + 4 * (lane >> 5) + (t >> 2);
+  const int p = 4 * dt + 2 * ((lane >> 4) & 1) + ((t & 3) >> 1);
+  const int in = (t & 1) << 3;
+  const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(tile + piece<D>(r, p) + in));
+  const s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(tile + piece<D>(r + 8, p) + in));
+  return __builtin_bit_cast(b8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+__device__ __forceinline__ f16 mfma(b8 a, b8 b, f16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+__device__ __forceinline__ int crow(int r, int hi) { return (r & 3) + 8 * (r >> 2) + 4 * hi; }
+
+// C's registers 8 ks .. 8 ks + 7 as the B fragment of k-step ks
+__device__ __forceinline__ b8 pack(const f16& c, int ks) {
+  b8 v;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = (__bf16)c[8 * ks + e];
+  return v;
+}
+
+// ---- staging of 64 rows of two matrices by 256 threads, through registers so
+// that rows that must not count (masked keys, rows past the end) become zero:
+// what stands there, NaN too, cannot reach a result.
+template <int D>
+struct Stage {
+  static constexpr int N = KC * D / 8 / 256;  // 16-byte pieces a thread, each matrix
+  b8 x[N], y[N];
+  bool on[N];
+
+  __device__ __forceinline__ static int row(int i) { return (threadIdx.x + 256 * i) / (D / 8); }
+  __device__ __forceinline__ static int col(int i) { return (threadIdx.x + 256 * i) % (D / 8); }
+
+  __device__ __forceinline__ void load(const __bf16* px, long long sx, const __bf16* py, long long sy, int r0, int end) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int r = min(r0 + row(i), end - 1);
+      x[i] = *(const b8*)(px + r * sx + col(i) * 8);
+      y[i] = *(const b8*)(py + r * sy + col(i) * 8);
+    }
+  }
+  __device__ __forceinline__ void store(char* tx, char* ty) {
+    const b8 zero = {};
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int at = piece<D>(row(i), col(i));
+      *(b8*)(tx + at) = on[i] ? x[i] : zero;
+      *(b8*)(ty + at) = on[i] ? y[i] : zero;
+    }
+  }
+};
+
+// ---- the bias of one head in LDS: entry x is the offset clamp(x - 3 - far),
+// copy c holds the entries from c on. `sign` -1: offsets mirrored.
+__device__ __forceinline__ int bias_len(int far) { return (2 * far + 10) & ~3; }
+
+// A table value of the type's lowest stands for a mask, as -inf does: divided
+// by the scale it would leave 32 bits' range, and a sum of exponentials of it
+// would be lost in the saved logarithm.
+__device__ __forceinline__ float as_bias(__bf16 t, float scale) {
+  const float f = (float)t;
+  return f < -3.38e38f ? -INF : f / scale;
+}
+
+__device__ __forceinline__ float bias_at(const RelArgs& a, int d, int h) {
+  const int n = min(max(a.map[d + a.far], 0), a.buckets - 1);
+  return as_bias(a.table[(long long)n * a.NH + h], a.scale);
+}
+
+__device__ void stage_bias(const RelArgs& a, int h, int sign, float* bias) {
+  const int len = bias_len(a.far);
+  for (int x = threadIdx.x; x < len + 3; x += 256) {
+    const int d = min(max(x - 3 - a.far, -a.far), a.far);
+    const float v = bias_at(a, sign * d, h);
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      if (x >= c && x - c < len) bias[c * len + x - c] = v;
+  }
+}
+
+// C's initial value for rows u0 + crow(r) against column w: the bias of the
+// offset row - column. `low`, `high`: the values beyond the largest distance.
+__device__ __forceinline__ f16 bias_tile(const float* bias, int far, int row0, int col0, int lane, float low, float high) {
+  f16 c;
+  if (row0 + 31 - col0 <= -far || row0 - (col0 + 31) >= far) {
+    const float v = row0 < col0 ? low : high;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) c[r] = v;
+    return c;
+  }
+  const int len = bias_len(far);
+  const int d = row0 + 4 * (lane >> 5) - (col0 + (lane & 31));
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const int x = min(max(d + 8 * g, -far - 3), far) + far + 3;
+    const f4 v = *(const f4*)(bias + (x & 3) * len + (x & ~3));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c[4 * g + e] = v[e];
+  }
+  return c;
+}
+
+// the workgroup's (batch and head, tile): neighbours in one XCD's share of the
+// ids (id mod 8) work on one head, so that its K and V stay in that XCD's L2
+__device__ __forceinline__ int remap(int id, int n) {
+  return (n & 7) ? id : (id & 7) * (n >> 3) + (id >> 3);
+}
+
+// one past the last key that the mask leaves, 0 if it leaves none. All threads.
+__device__ int mask_end(const unsigned char* mask, int end, int* lds) {
+  int last = 0;
+  for (int j = threadIdx.x; j < end; j += 256)
+    if (mask[j]) last = j + 1;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) last = max(last, __shfl_xor(last, o, 64));
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = last;
+  __syncthreads();
+  last = max(max(lds[0], lds[1]), max(lds[2], lds[3]));
+  return last;
+}
+
+// which of a chunk's 64 keys count, one bit each
+__device__ __forceinline__ unsigned long long key_bits(const unsigned char* mask, int j0, int end) {
+  const int j = j0 + (threadIdx.x & 63);
+  const bool on = j < end && (!mask || mask[min(j, end - 1)]);
+  return __ballot(on);
+}
+
+// C rows whose key does not count, or lies behind the column's query -> fill
+__device__ __forceinline__ void drop_rows(f16& c, unsigned bits, bool diag, int key0, int query0, int lane, float fill) {
+  const int hi = lane >> 5;
+  if (bits != ~0u) {
+    const unsigned b = bits >> (4 * hi);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) c[r] = (b >> crow(r, 0)) & 1 ? c[r] : fill;
+  }
+  if (diag) {
+    const int most = query0 + (lane & 31) - key0 - 4 * hi;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) c[r] = crow(r, 0) <= most ? c[r] : fill;
+  }
+}
+
+template <int D>
+__device__ __forceinline__ void store_columns(__bf16* row, const f16* c, float mul, int hi) {
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      b4 v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = (__bf16)(c[dt][4 * g + e] * mul);
+      *(b4*)(row + 32 * dt + 8 * g + 4 * hi) = v;
+    }
+}
+
+// ---------------- forward: a wave owns 32 queries, chunks of 64 keys ----------------
+template <int D>
+__global__ __launch_bounds__(256) void k_rel_fwd(RelArgs a, int tiles) {
+  extern __shared__ __align__(16) char smem[];
+  __shared__ int ends[4];
+  char* buf = smem;  // [2][K, V]
+  constexpr int MAT = KC * 2 * D;
+  float* bias = (float*)(smem + 4 * MAT);
+
+  const int id = remap(blockIdx.x, gridDim.x);
+  const int bh = id / tiles, h = bh % a.NH, b = bh / a.NH, hk = h / (a.NH / a.NKV);
+  const int tile = a.causal ? tiles - 1 - id % tiles : id % tiles;
+  const int lane = threadIdx.x & 63, hi = lane >> 5;
+  const int i0 = tile * TILE + (threadIdx.x >> 6) * 32, i = i0 + (lane & 31);
+  const __bf16* k = a.k + b * a.k_b + hk * a.k_h;
+  const __bf16* v = a.v + b * a.v_b + hk * a.v_h;
+  const unsigned char* mask = a.mask ? a.mask + (long long)b * a.S : nullptr;
+
+  stage_bias(a, h, 1, bias);
+  int end = a.causal ? min(a.S, tile * TILE + TILE) : a.S;
+  if (mask) end = mask_end(mask, end, ends);
+  const int chunks = (end + KC - 1) / KC;
+
+  b8 q[D / 16];
+  const __bf16* qp = a.q + b * a.q_b + min(i, a.S - 1) * a.q_s + h * a.q_h;
+#pragma unroll
+  for (int t = 0; t < D / 16; ++t) q[t] = *(const b8*)(qp + 16 * t + 8 * hi);
+
+  f16 o[D / 32] = {};
+  float m = -INF, l = 0.f;
+  const float c2 = a.scale * LOG2E;
+
+  Stage<D> st;
+  unsigned long long bits = 0, next = 0;
+  auto fetch = [&](int c) {
+    st.load(k, a.k_s, v, a.v_s, c * KC, end);
+    next = key_bits(mask, c * KC, end);
+#pragma unroll
+    for (int n = 0; n < Stage<D>::N; ++n) st.on[n] = (next >> Stage<D>::row(n)) & 1;
+  };
+  if (chunks > 0) {
+    fetch(0);
+    st.store(buf, buf + MAT);
+  }
+  __syncthreads();
+  const float low = bias[0], high = bias[2 * a.far + 3];
+
+  for (int c = 0; c < chunks; ++c) {
+    bits = next;
+    if (c + 1 < chunks) fetch(c + 1);
+    if (c > 0) __syncthreads();
+    const char* kt = buf + (c & 1) * 2 * MAT;
+    const char* vt = kt + MAT;
+#pragma unroll
+    for (int sub = 0; sub < 2; ++sub) {
+      const int j0 = c * KC + 32 * sub;
+      const unsigned on = (unsigned)(bits >> (32 * sub));
+      if (on == 0 || (a.causal && j0 > i0 + 31)) continue;
+      f16 s = bias_tile(bias, a.far, j0, i0, lane, low, high);
+#pragma unroll
+      for (int t = 0; t < D / 16; ++t) s = mfma(row_frag<D>(kt, 32 * sub + (lane & 31), t, hi), q[t], s);
+      drop_rows(s, on, a.causal && j0 + 31 > i0, j0, i0, lane, -INF);
+      float top = s[0];
+#pragma unroll
+      for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
+      top = fmaxf(top, __shfl_xor(top, 32, 64)) * c2;
+      // the maximum moves only where it grew by more than 8 (a factor of 256,
+      // far inside 32 bits and the same relative rounding in bf16): after the
+      // first chunks the accumulators are hardly ever rescaled
+      if (__any(top > m + 8.f)) {
+        const float n = fmaxf(m, top);
+        const float f = n == -INF ? 1.f : __builtin_amdgcn_exp2f(m - n);
+        m = n;
+        l *= f;
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[dt][r] *= f;
+      }
+      const float base = m == -INF ? 0.f : m;
+      float sum = 0.f;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c2, -base));
+        sum += s[r];
+      }
+      l += sum;
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        const b8 p = pack(s, ks);
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt) o[dt] = mfma(col_frag<D>(vt, 32 * sub + 16 * ks, dt, lane), p, o[dt]);
+      }
+    }
+    if (c + 1 < chunks) {
+      char* to = buf + ((c + 1) & 1) * 2 * MAT;
+      st.store(to, to + MAT);
+    }
+  }
+  l += __shfl_xor(l, 32, 64);
+  if (i >= a.S) return;
+  store_columns<D>(a.out + (((long long)b * a.S + i) * a.NH + h) * D, o, l == 0.f ? 0.f : 1.f / l, hi);
+  if (a.lse && hi == 0) a.lse[(long long)bh * a.S + i] = l == 0.f ? INF : m + __builtin_amdgcn_logf(l);
+}
+
+// ---------------- backward 1: dQ, D and the offsets' sums of dS ----------------
+template <int D>
+__global__ __launch_bounds__(256) void k_rel_bwd_q(RelArgs a, int tiles) {
+  extern __shared__ __align__(16) char smem[];
+  __shared__ int ends[4];
+  char* buf = smem;  // [2][K, V]
+  constexpr int MAT = KC * 2 * D;
+  float* bias = (float*)(smem + 4 * MAT);
+  const int offs = 2 * a.far + 1;
+  float* sums = bias + 4 * bias_len(a.far);  // [4 waves][offs]
+
+  const int id = remap(blockIdx.x, gridDim.x);
+  const int bh = id / tiles, h = bh % a.NH, b = bh / a.NH, hk = h / (a.NH / a.NKV);
+  const int tile = a.causal ? tiles - 1 - id % tiles : id % tiles;
+  const int lane = threadIdx.x & 63, hi = lane >> 5, wave = threadIdx.x >> 6;
+  const int i0 = tile * TILE + wave * 32, i = i0 + (lane & 31);
+  const __bf16* k = a.k + b * a.k_b + hk * a.k_h;
+  const __bf16* v = a.v + b * a.v_b + hk * a.v_h;
+  const unsigned char* mask = a.mask ? a.mask + (long long)b * a.S : nullptr;
+
+  stage_bias(a, h, 1, bias);
+  for (int x = threadIdx.x; x < 4 * offs; x += 256) sums[x] = 0.f;
+  int end = a.causal ? min(a.S, tile * TILE + TILE) : a.S;
+  if (mask) end = mask_end(mask, end, ends);
+  const int chunks = (end + KC - 1) / KC;
+
+  // a row past the end, or with nothing allowed, takes part as zeros
+  const float lse = i < a.S ? a.lse[(long long)bh * a.S + i] : INF;
+  const bool live = lse < INF || lse != lse;
+  b8 q[D / 16], g[D / 16];
+  float dsum = 0.f;
+  {
+    const int r = min(i, a.S - 1);
+    const __bf16* qp = a.q + b * a.q_b + r * a.q_s + h * a.q_h;
+    const long long at = (((long long)b * a.S + r) * a.NH + h) * D;
+    const b8 zero = {};
+#pragma unroll
+    for (int t = 0; t < D / 16; ++t) {
+      q[t] = *(const b8*)(qp + 16 * t + 8 * hi);
+      g[t] = *(const b8*)(a.dout + at + 16 * t + 8 * hi);
+      const b8 out = *(const b8*)(a.out + at + 16 * t + 8 * hi);
+      q[t] = live ? q[t] : zero;
+      g[t] = live ? g[t] : zero;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) dsum = fmaf((float)g[t][e], (float)out[e], dsum);
+    }
+  }
+  dsum += __shfl_xor(dsum, 32, 64);
+  if (i < a.S && hi == 0) a.dsum[(long long)bh * a.S + i] = dsum;
+
+  f16 dq[D / 32] = {};
+  const float c2 = a.scale * LOG2E;
+  float* mine = sums + wave * offs;
+  float far_low = 0.f, far_high = 0.f;
+
+  Stage<D> st;
+  unsigned long long bits = 0, next = 0;
+  auto fetch = [&](int c) {
+    st.load(k, a.k_s, v, a.v_s, c * KC, end);
+    next = key_bits(mask, c * KC, end);
+#pragma unroll
+    for (int n = 0; n < Stage<D>::N; ++n) st.on[n] = (next >> Stage<D>::row(n)) & 1;
+  };
+  if (chunks > 0) {
+    fetch(0);
+    st.store(buf, buf + MAT);
+  }
+  __syncthreads();
+  const float low = bias[0], high = bias[2 * a.far + 3];
+
+  for (int c = 0; c < chunks; ++c) {
+    bits = next;
+    if (c + 1 < chunks) fetch(c + 1);
+    if (c > 0) __syncthreads();
+    const char* kt = buf + (c & 1) * 2 * MAT;
+    const char* vt = kt + MAT;
+#pragma unroll
+    for (int sub = 0; sub < 2; ++sub) {
+      const int j0 = c * KC + 32 * sub;
+      const unsigned on = (unsigned)(bits >> (32 * sub));
+      if (on == 0 || (a.causal && j0 > i0 + 31)) continue;
+      f16 s = bias_tile(bias, a.far, j0, i0, lane, low, high);
+      f16 dp = {};
+#pragma unroll
+      for (int t = 0; t < D / 16; ++t) {
+        s = mfma(row_frag<D>(kt, 32 * sub + (lane & 31), t, hi), q[t], s);
+        dp = mfma(row_frag<D>(vt, 32 * sub + (lane & 31), t, hi), g[t], dp);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c2, -lse)) * (dp[r] - dsum);
+      drop_rows(s, on, a.causal && j0 + 31 > i0, j0, i0, lane, 0.f);
+      // sums of dS by offset: tiles beyond the largest distance in a register,
+      // others by LDS additions into the wave's own array (a wave's additions
+      // are made in order, so the result does not depend on timing)
+      if (j0 + 31 - i0 <= -a.far || j0 - (i0 + 31) >= a.far) {
+        float t = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) t += s[r];
+        if (j0 < i0) far_low += t;
+        else far_high += t;
+      } else {
+        const int d = j0 + 4 * hi - i;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int x = min(max(d + crow(r, 0), -a.far), a.far) + a.far;
+          __hip_atomic_fetch_add(mine + x, s[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        }
+      }
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        const b8 p = pack(s, ks);
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt) dq[dt] = mfma(col_frag<D>(kt, 32 * sub + 16 * ks, dt, lane), p, dq[dt]);
+      }
+    }
+    if (c + 1 < chunks) {
+      char* to = buf + ((c + 1) & 1) * 2 * MAT;
+      st.store(to, to + MAT);
+    }
+  }
+  if (i < a.S)
+    store_columns<D>(a.dq + b * a.dq_b + i * a.dq_s + (long long)h * D, dq, a.scale, hi);
+#pragma unroll
+  for (int x = 32; x > 0; x >>= 1) {
+    far_low += __shfl_xor(far_low, x, 64);
+    far_high += __shfl_xor(far_high, x, 64);
+  }
+  if (lane == 0) {
+    mine[0] += far_low;
+    mine[offs - 1] += far_high;
+  }
+  __syncthreads();
+  float* to = a.doff + ((long long)bh * tiles + tile) * offs;
+  for (int x = threadIdx.x; x < offs; x += 256)
+    to[x] = (sums[x] + sums[offs + x]) + (sums[2 * offs + x] + sums[3 * offs + x]);
+}
+
+// ---------------- backward 2: dK and dV; a wave owns 32 keys, chunks of 64 queries ----------------
+template <int D>
+__global__ __launch_bounds__(256) void k_rel_bwd_kv(RelArgs a, int tiles) {
+  extern __shared__ __align__(16) char smem[];
+  char* buf = smem;  // [2][Q, dO]
+  constexpr int MAT = KC * 2 * D;
+  float* rows = (float*)(smem + 4 * MAT);  // [2][lse, D][64]
+  float* bias = rows + 4 * KC;
+
+  const int id = remap(blockIdx.x, gridDim.x);
+  const int bk = id / tiles, hk = bk % a.NKV, b = bk / a.NKV, group = a.NH / a.NKV;
+  const int tile = id % tiles;
+  const int lane = threadIdx.x & 63, hi = lane >> 5;
+  const int j0 = tile * TILE + (threadIdx.x >> 6) * 32, j = j0 + (lane & 31);
+  const bool keep = j < a.S && (!a.mask || a.mask[(long long)b * a.S + min(j, a.S - 1)]);
+  const bool work = __any(keep);  // this wave has a key that counts
+
+  b8 k[D / 16], v[D / 16];
+  {
+    const int r = min(j, a.S - 1);
+    const __bf16* kp = a.k + b * a.k_b + r * a.k_s + hk * a.k_h;
+    const __bf16* vp = a.v + b * a.v_b + r * a.v_s + hk * a.v_h;
+    const b8 zero = {};
+#pragma unroll
+    for (int t = 0; t < D / 16; ++t) {
+      k[t] = *(const b8*)(kp + 16 * t + 8 * hi);
+      v[t] = *(const b8*)(vp + 16 * t + 8 * hi);
+      k[t] = keep ? k[t] : zero;
+      v[t] = keep ? v[t] : zero;
+    }
+  }
+  f16 dk[D / 32] = {}, dv[D / 32] = {};
+  const float c2 = a.scale * LOG2E;
+  const int first = a.causal ? tile * TILE / KC : 0, chunks = (a.S + KC - 1) / KC;
+  Stage<D> st;
+  float row_lse = 0.f, row_d = 0.f;
+
+  if (__syncthreads_or(work))
+    for (int n = 0; n < group; ++n) {
+      const int h = hk * group + n, bh = b * a.NH + h;
+      const __bf16* q = a.q + b * a.q_b + h * a.q_h;
+      const __bf16* g = a.dout + ((long long)b * a.S * a.NH + h) * D;
+      const long long g_s = (long long)a.NH * D;
+      const float* lse = a.lse + (long long)bh * a.S;
+      const float* dsum = a.dsum + (long long)bh * a.S;
+      auto fetch = [&](int c) {
+        st.load(q, a.q_s, g, g_s, c * KC, a.S);
+#pragma unroll
+        for (int x = 0; x < Stage<D>::N; ++x) {
+          const int r = c * KC + Stage<D>::row(x);
+          const float e = r < a.S ? lse[r] : INF;
+          st.on[x] = e < INF || e != e;  // rows past the end or with nothing allowed: zeros
+        }
+        if (threadIdx.x < KC) {
+          const int r = c * KC + threadIdx.x;
+          row_lse = r < a.S ? lse[r] : INF;
+          row_d = r < a.S ? dsum[r] : 0.f;
+        }
+      };
+      auto put = [&](int c) {
+        char* to = buf + (c & 1) * 2 * MAT;
+        st.store(to, to + MAT);
+        if (threadIdx.x < KC) {
+          float* r = rows + (c & 1) * 2 * KC;
+          r[threadIdx.x] = row_lse;
+          r[KC + threadIdx.x] = row_d;
+        }
+      };
+      __syncthreads();  // the last head's tiles are read
+      stage_bias(a, h, -1, bias);
+      fetch(first);
+      put(first);
+      __syncthreads();
+      const float low = bias[0], high = bias[2 * a.far + 3];
+      for (int c = first; c < chunks; ++c) {
+        if (c + 1 < chunks) fetch(c + 1);
+        if (c > first) __syncthreads();
+        const char* qt = buf + (c & 1) * 2 * MAT;
+        const char* gt = qt + MAT;
+        const float* rl = rows + (c & 1) * 2 * KC;
+        if (work)
+#pragma unroll
+          for (int sub = 0; sub < 2; ++sub) {
+            const int i0 = c * KC + 32 * sub;
+            if (i0 >= a.S || (a.causal && i0 + 31 < j0)) continue;
+            // rows are queries here: the mirrored bias of row - column
+            f16 s = bias_tile(bias, a.far, i0, j0, lane, low, high);
+            f16 dp = {};
+#pragma unroll
+            for (int t = 0; t < D / 16; ++t) {
+              s = mfma(row_frag<D>(qt, 32 * sub + (lane & 31), t, hi), k[t], s);
+              dp = mfma(row_frag<D>(gt, 32 * sub + (lane & 31), t, hi), v[t], dp);
+            }
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const f4 e = *(const f4*)(rl + 32 * sub + 8 * x + 4 * hi);
+              const f4 d = *(const f4*)(rl + KC + 32 * sub + 8 * x + 4 * hi);
+#pragma unroll
+              for (int y = 0; y < 4; ++y) {
+                const int r = 4 * x + y;
+                s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c2, -e[y]));
+                dp[r] = dp[r] - d[y];
+              }
+            }
+            if (a.causal && i0 < j0 + 31) {
+              const int least = j - i0 - 4 * hi;
+#pragma unroll
+              for (int r = 0; r < 16; ++r) s[r] = crow(r, 0) >= least ? s[r] : 0.f;
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) dp[r] *= s[r];
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+              const b8 p = pack(s, ks), ds = pack(dp, ks);
+#pragma unroll
+              for (int dt = 0; dt < D / 32; ++dt) {
+                dv[dt] = mfma(col_frag<D>(gt, 32 * sub + 16 * ks, dt, lane), p, dv[dt]);
+                dk[dt] = mfma(col_frag<D>(qt, 32 * sub + 16 * ks, dt, lane), ds, dk[dt]);
+              }
+            }
+          }
+        if (c + 1 < chunks) put(c + 1);
+      }
+    }
+  if (j >= a.S) return;
+  // a masked key's column holds what its zeroed K and V gave: it has no gradient
+  const f16 none[D / 32] = {};
+  const long long at = b * a.dk_b + j * a.dk_s + (long long)hk * D;
+  store_columns<D>(a.dk + at, keep ? dk : none, a.scale, hi);
+  store_columns<D>(a.dv + at, keep ? dv : none, 1.f, hi);
+}
+
+// dtable[n][h]: the offsets' sums over batches and tiles, then over the offsets
+// of a bucket; one workgroup a head, every sum in a fixed order.
+__global__ __launch_bounds__(1024) void k_rel_dtable(RelArgs a, int tiles) {
+  __shared__ float part[4][256];
+  __shared__ float sums[2 * GA_REL_MAX_DISTANCE + 1];
+  const int h = blockIdx.x, offs = 2 * a.far + 1, x = threadIdx.x & 255, y = threadIdx.x >> 8;
+  const int n = a.B * tiles;
+  for (int x0 = 0; x0 < offs; x0 += 256) {
+    float t = 0.f;
+    if (x0 + x < offs)
+      for (int w = y; w < n; w += 4)
+        t += a.doff[((long long)(w / tiles * a.NH + h) * tiles + w % tiles) * offs + x0 + x];
+    part[y][x] = t;
+    __syncthreads();
+    if (y == 0 && x0 + x < offs) sums[x0 + x] = (part[0][x] + part[1][x]) + (part[2][x] + part[3][x]);
+    __syncthreads();
+  }
+  const int lane = threadIdx.x & 63;
+  for (int bucket = threadIdx.x >> 6; bucket < a.buckets; bucket += 16) {
+    float t = 0.f;
+    for (int e = lane; e < offs; e += 64)
+      if (min(max(a.map[e], 0), a.buckets - 1) == bucket) t += sums[e];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) t += __shfl_xor(t, o, 64);
+    if (lane == 0) a.dtable[(long long)bucket * a.NH + h] = (__bf16)t;
+  }
+}
+
+// ---------------- new tokens over a cache ----------------
+// The columns of a wave's tile are the rows (new token, head of the group) that
+// share a key/value head: one read of K and V serves them all. The keys are
+// split over `splits` workgroups and four waves each; a wave takes 32 keys at a
+// time, K straight into A fragments, V through its own LDS tile. The waves'
+// (maximum, sum, output) are joined in LDS, the workgroups' by k_rel_join.
+template <int D>
+__global__ __launch_bounds__(256) void k_rel_token(RelTokenArgs a, int row_tiles) {
+  extern __shared__ __align__(16) char smem[];
+  const int lane = threadIdx.x & 63, hi = lane >> 5, wave = threadIdx.x >> 6;
+  const int group = a.NH / a.NKV, rows = group * a.Sq;
+  const int split = blockIdx.x % a.splits, rest = blockIdx.x / a.splits;
+  const int rt = rest % row_tiles, hk = rest / row_tiles % a.NKV, b = rest / row_tiles / a.NKV;
+  constexpr int MAT = 32 * 2 * D;
+  char* vt = smem + wave * MAT;
+  int* map = (int*)(smem + 4 * MAT);             // [far + 1], offsets -far .. 0
+  float* table = (float*)(map + a.far + 1);      // [buckets][heads of this tile]
+  const int row = rt * 32 + (lane & 31);
+  const int tok = min(row, rows - 1) / group, h = hk * group + min(row, rows - 1) % group;
+  const int len = min(max(a.lengths[b], 0), a.S);
+  const int pos = row < rows ? len - a.Sq + tok : -1;  // the last key of this row
+  const int pos0 = len - a.Sq + rt * 32 / group;       // the first row's
+
+  for (int x = threadIdx.x; x <= a.far; x += 256) map[x] = min(max(a.map[x], 0), a.buckets - 1);
+  for (int x = threadIdx.x; x < a.buckets * group; x += 256)
+    table[x] = as_bias(a.table[(long long)(x / group) * a.NH + hk * group + x % group], a.scale);
+
+  b8 q[D / 16];
+  const __bf16* qp = a.q + b * a.q_b + tok * a.q_s + h * a.q_h;
+#pragma unroll
+  for (int t = 0; t < D / 16; ++t) q[t] = *(const b8*)(qp + 16 * t + 8 * hi);
+  __syncthreads();
+  const int mine = h - hk * group;
+  const float low = table[map[0] * group + mine];
+
+  // keys in units of 32, spread evenly over the waves of all splits
+  const int units = (len + 31) / 32, waves = a.splits * 4, w = split * 4 + wave;
+  const int u0 = (int)((long long)units * w / waves), u1 = (int)((long long)units * (w + 1) / waves);
+  const __bf16* k = a.k + b * a.k_b + hk * a.k_h;
+  const __bf16* v = a.v + b * a.v_b + hk * a.v_h;
+  constexpr int NV = 32 * D / 8 / 64;
+  b8 kf[D / 16], vf[NV];
+  auto fetch = [&](int u) {
+    const int j = u * 32 + (lane & 31);
+    const __bf16* kp = k + min(j, len - 1) * a.k_s;
+#pragma unroll
+    for (int t = 0; t < D / 16; ++t) kf[t] = *(const b8*)(kp + 16 * t + 8 * hi);
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      const int x = lane + 64 * n, r = u * 32 + x / (D / 8);
+      vf[n] = *(const b8*)(v + min(r, len - 1) * a.v_s + x % (D / 8) * 8);
+    }
+  };
+  f16 o[D / 32] = {};
+  float m = -INF, l = 0.f;
+  const float c2 = a.scale * LOG2E;
+  if (u0 < u1) fetch(u0);
+  for (int u = u0; u < u1; ++u) {
+    const int j0 = u * 32;
+    const b8 zero = {};
+    f16 s;
+    if (j0 + 31 - pos0 <= -a.far) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = low;
+    } else {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int d = j0 + crow(r, hi) - pos;
+        s[r] = table[map[min(max(d, -a.far), 0) + a.far] * group + mine];
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < D / 16; ++t) {
+      const b8 f = j0 + (lane & 31) < len ? kf[t] : zero;
+      s = mfma(f, q[t], s);
+    }
+    // this tile's V into LDS; the wave alone reads it
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      const int x = lane + 64 * n, r = x / (D / 8);
+      *(b8*)(vt + piece<D>(r, x % (D / 8))) = j0 + r < len ? vf[n] : zero;
+    }
+    if (u + 1 < u1) fetch(u + 1);
+    if (j0 + 31 > pos0) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = j0 + crow(r, hi) <= pos ? s[r] : -INF;
+    }
+    float top = s[0];
+#pragma unroll
+    for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
+    top = fmaxf(top, __shfl_xor(top, 32, 64)) * c2;
+    if (__any(top > m + 8.f)) {
+      const float n = fmaxf(m, top);
+      const float f = n == -INF ? 1.f : __builtin_amdgcn_exp2f(m - n);
+      m = n;
+      l *= f;
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[dt][r] *= f;
+    }
+    const float base = m == -INF ? 0.f : m;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c2, -base));
+      l += s[r];
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      const b8 p = pack(s, ks);
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt) o[dt] = mfma(col_frag<D>(vt, 16 * ks, dt, lane), p, o[dt]);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+  l += __shfl_xor(l, 32, 64);
+
+  // join the four waves: [4][32 rows][maximum, sum], then [32][D] by turns
+  __syncthreads();
+  float* stat = (float*)smem;          // [4][2][32]
+  float* acc = (float*)smem + 4 * 64;  // [32][D + 1]
+  if (hi == 0) {
+    stat[wave * 64 + lane] = m;
+    stat[wave * 64 + 32 + lane] = l;
+  }
+  __syncthreads();
+  const int x = lane & 31;
+  float top = -INF, sum = 0.f;
+#pragma unroll
+  for (int n = 0; n < 4; ++n) top = fmaxf(top, stat[n * 64 + x]);
+  const float base = top == -INF ? 0.f : top;
+#pragma unroll
+  for (int n = 0; n < 4; ++n) sum += stat[n * 64 + 32 + x] * __builtin_amdgcn_exp2f(stat[n * 64 + x] - base);
+  const float f = __builtin_amdgcn_exp2f(m - base);
+  for (int n = 0; n < 4; ++n) {
+    if (wave == n)
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          float* p = acc + x * (D + 1) + 32 * dt + crow(r, hi);
+          *p = n == 0 ? o[dt][r] * f : *p + o[dt][r] * f;
+        }
+    __syncthreads();
+  }
+  float* stats = (float*)smem;  // rows' maximum and sum, read by all below
+  if (threadIdx.x < 32) {
+    stats[threadIdx.x] = top;
+    stats[32 + threadIdx.x] = sum;
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < 32 * D; e += 256) {
+    const int r = e / D, d = e % D, at = rt * 32 + r;
+    if (at >= rows) continue;
+    if (a.splits == 1) {
+      const float z = stats[32 + r];
+      a.out[(((long long)b * a.Sq + at / group) * a.NH + hk * group + at % group) * D + d] =
+          (__bf16)(z == 0.f ? 0.f : acc[r * (D + 1) + d] / z);
+    } else {
+      float* p = a.parts + (((long long)rest * a.splits + split) * 32 + r) * (D + 2);
+      p[d] = acc[r * (D + 1) + d];
+      if (d == 0) {
+        p[D] = stats[r];
+        p[D + 1] = stats[32 + r];
+      }
+    }
+  }
+}
+
+// joins the workgroups' parts of one output row, in order
+template <int D>
+__global__ __launch_bounds__(D) void k_rel_join(RelTokenArgs a, int row_tiles) {
+  const int group = a.NH / a.NKV, rows = group * a.Sq;
+  const int at = blockIdx.x % rows, hk = blockIdx.x / rows % a.NKV, b = blockIdx.x / rows / a.NKV;
+  const long long rest = ((long long)b * a.NKV + hk) * row_tiles + at / 32;
+  const float* p = a.parts + (rest * a.splits * 32 + at % 32) * (D + 2);
+  const long long step = 32 * (D + 2);
+  float top = -INF;
+  for (int n = 0; n < a.splits; ++n) top = fmaxf(top, p[n * step + D]);
+  const float base = top == -INF ? 0.f : top;
+  float z = 0.f, o = 0.f;
+  for (int n = 0; n < a.splits; ++n) {
+    const float f = __builtin_amdgcn_exp2f(p[n * step + D] - base);
+    z = fmaf(p[n * step + D + 1], f, z);
+    o = fmaf(p[n * step + threadIdx.x], f, o);
+  }
+  a.out[(((long long)b * a.Sq + at / group) * a.NH + hk * group + at % group) * D + threadIdx.x] =
+      (__bf16)(z == 0.f ? 0.f : o / z);
+}
+
+size_t bias_bytes(int far) { return 16 * (size_t)((2 * far + 10) & ~3); }
+
+// dynamic LDS above 64 KB has to be asked for
+template <typename F>
+hipError_t allow(F* f, size_t bytes) {
+  if (bytes <= 64 * 1024) return hipSuccess;
+  return hipFuncSetAttribute((const void*)f, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+}
+
+template <int D>
+hipError_t forward(const RelArgs& a, hipStream_t s) {
+  const int tiles = rel_tiles(a.S);
+  const size_t lds = 4 * KC * 2 * D + bias_bytes(a.far);
+  const hipError_t e = allow(k_rel_fwd<D>, lds);
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL((k_rel_fwd<D>), dim3(a.B * a.NH * tiles), dim3(256), lds, s, a, tiles);
+  return hipGetLastError();
+}
+
+template <int D>
+hipError_t backward(const RelArgs& a, hipStream_t s) {
+  const int tiles = rel_tiles(a.S);
+  const size_t lds_q = 4 * KC * 2 * D + bias_bytes(a.far) + 16 * (2 * a.far + 1);
+  const size_t lds_kv = 4 * KC * 2 * D + 16 * KC + bias_bytes(a.far);
+  hipError_t e = allow(k_rel_bwd_q<D>, lds_q);
+  if (e == hipSuccess) e = allow(k_rel_bwd_kv<D>, lds_kv);
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL((k_rel_bwd_q<D>), dim3(a.B * a.NH * tiles), dim3(256), lds_q, s, a, tiles);
+  if ((e = hipGetLastError()) != hipSuccess) return e;
+  hipLaunchKernelGGL((k_rel_bwd_kv<D>), dim3(a.B * a.NKV * tiles), dim3(256), lds_kv, s, a, tiles);
+  if ((e = hipGetLastError()) != hipSuccess) return e;
+  hipLaunchKernelGGL(k_rel_dtable, dim3(a.NH), dim3(1024), 0, s, a, tiles);
+  return hipGetLastError();
+}
+
+template <int D>
+hipError_t token(const RelTokenArgs& a, hipStream_t s) {
+  const int group = a.NH / a.NKV, rows = group * a.Sq, row_tiles = (rows + 31) / 32;
+  size_t lds = 4 * 32 * 2 * D + 4 * (a.far + 1) + 4 * (size_t)a.buckets * group;
+  const size_t join = 4 * (4 * 64 + 32 * (D + 1));
+  if (lds < join) lds = join;
+  const hipError_t e = allow(k_rel_token<D>, lds);
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL((k_rel_token<D>), dim3(a.B * a.NKV * row_tiles * a.splits), dim3(256), lds, s, a, row_tiles);
+  if (a.splits > 1) hipLaunchKernelGGL((k_rel_join<D>), dim3(a.B * a.NKV * rows), dim3(D), 0, s, a, row_tiles);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+int rel_tiles(int S) { return (S + TILE - 1) / TILE; }
+
+// enough workgroups to fill the chip twice, but at least 128 keys a wave
+int rel_token_splits(int B, int Sq, int S, int NH, int NKV) {
+  const long long rows = (long long)(NH / NKV) * Sq, base = (long long)B * NKV * ((rows + 31) / 32);
+  long long n = (512 + base - 1) / base;
+  const long long most = (S + 511) / 512;
+  if (n > most) n = most;
+  return (int)(n < 1 ? 1 : n);
+}
+
+hipError_t rel_forward(const RelArgs& a, hipStream_t s) { return a.D == 64 ? forward<64>(a, s) : forward<128>(a, s); }
+hipError_t rel_backward(const RelArgs& a, hipStream_t s) { return a.D == 64 ? backward<64>(a, s) : backward<128>(a, s); }
+hipError_t rel_token(const RelTokenArgs& a, hipStream_t s) { return a.D == 64 ? token<64>(a, s) : token<128>(a, s); }

@@ -41,6 +41,7 @@ setup(
                 os.path.join(CSRC, "linear_small.hip"),
                 os.path.join(CSRC, "rms_norm.hip"),
                 os.path.join(CSRC, "grad_clip.hip"),
+                os.path.join(CSRC, "rel_attn.hip"),
                 os.path.join(CSRC, "ops_bindings.hip"),
                 os.path.join(CSRC, "ga_bindings.hip"),
             ],

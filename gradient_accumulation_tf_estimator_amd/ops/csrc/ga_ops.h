@@ -45,7 +45,7 @@ hipError_t clip_finish(const double* sums, int n, double clip, float* norm, floa
 hipError_t clip_scale(const ClipArgs& a, const float* coef, hipStream_t s);
 
 // ---- attention with a relative position bias (rel_attn.hip); strides in elements ----
-#define GA_REL_MAX_DISTANCE 1024
+#define GA_REL_MAX_DISTANCE 512
 #define GA_REL_MAX_BUCKETS 256
 struct RelArgs {
   const __bf16 *q, *k, *v;

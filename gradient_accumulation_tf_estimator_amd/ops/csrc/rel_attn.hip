@@ -329,6 +329,27 @@ __global__ __launch_bounds__(256) void k_rel_fwd(RelArgs a, int tiles) {
   if (a.lse && hi == 0) a.lse[(long long)bh * a.S + i] = l == 0.f ? INF : m + __builtin_amdgcn_logf(l);
 }
 
+// lane i of each 16 takes lane i + N's value (N < 0: i - |N|), zero from outside
+template <int N>
+__device__ __forceinline__ float from_lane(float x) {
+  if (N == 0) return x;
+  constexpr int how = N > 0 ? 0x100 + N : 0x110 - N;
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), how, 0xf, 0xf, true));
+}
+
+// Sums of a 32x32 tile along its diagonals. In register r of a lane stands row
+// 16 u + s + 4 hi (s = r & 3 | 8 (r >> 2 & 1), u = r >> 3), column 16 ib + i.
+// Moved s lanes down within the 16, every register's lane holds the same
+// offset but for a multiple of 16, so the additions are plain: d[n] of lane i
+// is the sum for the offset first - first column + 4 hi - 16 ib - i + 16 n.
+template <int R = 0>
+__device__ __forceinline__ void diagonals(const f16& c, float* d) {
+  constexpr int s = (R & 3) | ((R & 4) << 1), u = R >> 3;
+  d[u] += from_lane<s>(c[R]);
+  if (s) d[u + 1] += from_lane<s ? s - 16 : 0>(c[R]);
+  if constexpr (R < 15) diagonals<R + 1>(c, d);
+}
+
 // ---------------- backward 1: dQ, D and the offsets' sums of dS ----------------
 template <int D>
 __global__ __launch_bounds__(256) void k_rel_bwd_q(RelArgs a, int tiles) {
@@ -338,7 +359,7 @@ __global__ __launch_bounds__(256) void k_rel_bwd_q(RelArgs a, int tiles) {
   constexpr int MAT = KC * 2 * D;
   float* bias = (float*)(smem + 4 * MAT);
   const int offs = 2 * a.far + 1;
-  float* sums = bias + 4 * bias_len(a.far);  // [4 waves][offs]
+  float* sums = bias + 4 * bias_len(a.far);  // [4 waves][2 halves][offs]
 
   const int id = remap(blockIdx.x, gridDim.x);
   const int bh = id / tiles, h = bh % a.NH, b = bh / a.NH, hk = h / (a.NH / a.NKV);
@@ -350,7 +371,7 @@ __global__ __launch_bounds__(256) void k_rel_bwd_q(RelArgs a, int tiles) {
   const unsigned char* mask = a.mask ? a.mask + (long long)b * a.S : nullptr;
 
   stage_bias(a, h, 1, bias);
-  for (int x = threadIdx.x; x < 4 * offs; x += 256) sums[x] = 0.f;
+  for (int x = threadIdx.x; x < 8 * offs; x += 256) sums[x] = 0.f;
   int end = a.causal ? min(a.S, tile * TILE + TILE) : a.S;
   if (mask) end = mask_end(mask, end, ends);
   const int chunks = (end + KC - 1) / KC;
@@ -381,8 +402,15 @@ __global__ __launch_bounds__(256) void k_rel_bwd_q(RelArgs a, int tiles) {
 
   f16 dq[D / 32] = {};
   const float c2 = a.scale * LOG2E;
-  float* mine = sums + wave * offs;
+  float* mine = sums + (2 * wave + hi) * offs;
   float far_low = 0.f, far_high = 0.f;
+  // diagonals not yet added: the last of a tile is the first of the next one
+  float left = 0.f;
+  int left_at = 0;
+  const int lane_off = 4 * hi - (lane & 31);  // 4 hi - 16 ib - i
+  auto add = [&](int d, float x) {
+    __hip_atomic_fetch_add(mine + min(max(d, -a.far), a.far) + a.far, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+  };
 
   Stage<D> st;
   unsigned long long bits = 0, next = 0;
@@ -421,8 +449,10 @@ __global__ __launch_bounds__(256) void k_rel_bwd_q(RelArgs a, int tiles) {
       for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c2, -lse)) * (dp[r] - dsum);
       drop_rows(s, on, a.causal && j0 + 31 > i0, j0, i0, lane, 0.f);
       // sums of dS by offset: tiles beyond the largest distance in a register,
-      // others by LDS additions into the wave's own array (a wave's additions
-      // are made in order, so the result does not depend on timing)
+      // others along their diagonals, then by LDS additions into an array of
+      // this half wave's own (32 lanes, 32 offsets, no two at one address but
+      // where they are clamped; a wave's additions are made in order, so the
+      // result does not depend on timing)
       if (j0 + 31 - i0 <= -a.far || j0 - (i0 + 31) >= a.far) {
         float t = 0.f;
 #pragma unroll
@@ -430,12 +460,15 @@ __global__ __launch_bounds__(256) void k_rel_bwd_q(RelArgs a, int tiles) {
         if (j0 < i0) far_low += t;
         else far_high += t;
       } else {
-        const int d = j0 + 4 * hi - i;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int x = min(max(d + crow(r, 0), -a.far), a.far) + a.far;
-          __hip_atomic_fetch_add(mine + x, s[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-        }
+        const int d0 = j0 - i0 + lane_off;
+        float d[3] = {};
+        if (left_at == j0) d[0] = left;
+        else add(left_at - i0 + lane_off, left);
+        diagonals(s, d);
+        add(d0, d[0]);
+        add(d0 + 16, d[1]);
+        left = d[2];
+        left_at = j0 + 32;
       }
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks) {
@@ -451,6 +484,7 @@ __global__ __launch_bounds__(256) void k_rel_bwd_q(RelArgs a, int tiles) {
   }
   if (i < a.S)
     store_columns<D>(a.dq + b * a.dq_b + i * a.dq_s + (long long)h * D, dq, a.scale, hi);
+  add(left_at - i0 + lane_off, left);
 #pragma unroll
   for (int x = 32; x > 0; x >>= 1) {
     far_low += __shfl_xor(far_low, x, 64);
@@ -462,8 +496,12 @@ __global__ __launch_bounds__(256) void k_rel_bwd_q(RelArgs a, int tiles) {
   }
   __syncthreads();
   float* to = a.doff + ((long long)bh * tiles + tile) * offs;
-  for (int x = threadIdx.x; x < offs; x += 256)
-    to[x] = (sums[x] + sums[offs + x]) + (sums[2 * offs + x] + sums[3 * offs + x]);
+  for (int x = threadIdx.x; x < offs; x += 256) {
+    float t = 0.f;
+#pragma unroll
+    for (int n = 0; n < 8; ++n) t += sums[n * offs + x];
+    to[x] = t;
+  }
 }
 
 // ---------------- backward 2: dK and dV; a wave owns 32 keys, chunks of 64 queries ----------------
@@ -841,7 +879,7 @@ hipError_t forward(const RelArgs& a, hipStream_t s) {
 template <int D>
 hipError_t backward(const RelArgs& a, hipStream_t s) {
   const int tiles = rel_tiles(a.S);
-  const size_t lds_q = 4 * KC * 2 * D + bias_bytes(a.far) + 16 * (2 * a.far + 1);
+  const size_t lds_q = 4 * KC * 2 * D + bias_bytes(a.far) + 32 * (2 * a.far + 1);
   const size_t lds_kv = 4 * KC * 2 * D + 16 * KC + bias_bytes(a.far);
   hipError_t e = allow(k_rel_bwd_q<D>, lds_q);
   if (e == hipSuccess) e = allow(k_rel_bwd_kv<D>, lds_kv);

@@ -33,7 +33,7 @@ from torch.autograd.function import once_differentiable
 
 from . import require_hip
 
-MAX_DISTANCE = 1024
+MAX_DISTANCE = 512
 MAX_BUCKETS = 256
 _LOWEST = -3.38e38  # a table value from here down masks its offsets
 

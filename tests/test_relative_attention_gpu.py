@@ -159,7 +159,7 @@ def test_shared_heads(NH, NKV, causal):
     check(2, 150, NH, NKV, 64, causal, padded(2, 150, 60))
 
 
-@pytest.mark.parametrize("nb,far", [(4, 3), (8, 5), (32, 64), (64, 300), (256, 1024)])
+@pytest.mark.parametrize("nb,far", [(4, 3), (8, 5), (32, 64), (64, 300), (256, 512)])
 @pytest.mark.parametrize("causal", [False, True])
 @pytest.mark.parametrize("D", [64, 128])
 def test_bucket_tables(nb, far, causal, D):
@@ -358,7 +358,7 @@ def test_token_many_rows(Sq, NH, NKV):
 
 def test_token_strides_and_far_offsets():
     torch.manual_seed(21)
-    m = relative_position_buckets(32, 1000, False).cuda()
+    m = relative_position_buckets(32, 500, False).cuda()
     B, S, NKV, D = 2, 500, 2, 64
     both = rand(B, NKV, S, 2, D)  # heads first, keys and values interleaved
     k, v = both[:, :, :, 0].transpose(1, 2), both[:, :, :, 1].transpose(1, 2)

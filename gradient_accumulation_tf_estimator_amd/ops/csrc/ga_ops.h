@@ -48,8 +48,7 @@ hipError_t clip_scale(const ClipArgs& a, const float* coef, hipStream_t s);
 #define GA_REL_MAX_DISTANCE 512
 #define GA_REL_MAX_BUCKETS 256
 struct RelArgs {
-  const __bf16 *q, *k, *v;
-  long long q_b, q_s, q_h, k_b, k_s, k_h, v_b, v_s, v_h;
+  const __bf16* qkv;          // [B][S][width], width = (NH + 2 NKV) * D
   const __bf16* table;        // [buckets][NH]
   const int* map;             // [2 * far + 1], the bucket of each offset
   const unsigned char* mask;  // [B][S], 1 = attend, or null
@@ -58,11 +57,10 @@ struct RelArgs {
   // backward
   const __bf16* dout;         // [B][S][NH][D]
   float* dsum;                // [B][NH][S]
-  __bf16 *dq, *dk, *dv;       // strides of q, k and v below
-  long long dq_b, dq_s, dk_b, dk_s;  // heads lie D apart
+  __bf16* dqkv;               // like qkv
   float* doff;                // [B * NH * tiles][2 * far + 1], tiles = rel_tiles(S)
   __bf16* dtable;             // [buckets][NH]
-  int B, S, NH, NKV, D, buckets, far, causal;
+  int B, S, NH, NKV, D, width, buckets, far, causal;
   float scale;
 };
 int rel_tiles(int S);

@@ -262,18 +262,15 @@ RelArgs rel_args(const at::Tensor& qkv, int64_t NH, int64_t NKV, const at::Tenso
   check_heads(NH, NKV, D);
   check_bias(table, map, qkv, NH);
   TORCH_CHECK(scale > 0 && std::isfinite(scale), "scale must be positive and finite");
+  // a chunk of 64 rows is addressed by 32 bits from its start
+  TORCH_CHECK(qkv.size(2) <= (1 << 23), "too many heads");
   TORCH_CHECK(S < (1ll << 24) && B * NH * (S / 128 + 1) < (1ll << 31), "too many rows");
   if (mask)
     TORCH_CHECK(mask->device() == qkv.device() && mask->scalar_type() == at::kByte && mask->is_contiguous() &&
                 mask->dim() == 2 && mask->size(0) == B && mask->size(1) == S, "mask must be a contiguous u8 [B, S] tensor");
   RelArgs a = {};
-  const __bf16* p = (const __bf16*)qkv.data_ptr();
-  a.q = p;
-  a.k = p + NH * D;
-  a.v = p + (NH + NKV) * D;
-  a.q_b = a.k_b = a.v_b = S * qkv.size(2);
-  a.q_s = a.k_s = a.v_s = qkv.size(2);
-  a.q_h = a.k_h = a.v_h = D;
+  a.qkv = (const __bf16*)qkv.data_ptr();
+  a.width = (int)qkv.size(2);
   a.table = (const __bf16*)table.data_ptr();
   a.map = map.data_ptr<int>();
   a.mask = mask ? mask->data_ptr<unsigned char>() : nullptr;
@@ -329,11 +326,7 @@ std::vector<at::Tensor> rel_attn_bwd(at::Tensor dout, at::Tensor qkv, at::Tensor
   a.dsum = dsum.data_ptr<float>();
   a.doff = doff.data_ptr<float>();
   a.dtable = (__bf16*)dtable.data_ptr();
-  a.dq = (__bf16*)dqkv.data_ptr();
-  a.dk = a.dq + NH * a.D;
-  a.dv = a.dk + NKV * a.D;
-  a.dq_b = a.dk_b = a.q_b;
-  a.dq_s = a.dk_s = a.q_s;
+  a.dqkv = (__bf16*)dqkv.data_ptr();
   check_launch(rel_backward(a, stream_of(qkv)), "rel_attn_bwd");
   return {dqkv, dtable};
 }

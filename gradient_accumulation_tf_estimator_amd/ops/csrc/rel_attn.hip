@@ -47,13 +47,14 @@ typedef __attribute__((address_space(3))) s4 lds_s4;
 constexpr int KC = 64;     // rows of a staged chunk
 constexpr int TILE = 128;  // rows of a workgroup: four waves of 32
 
-// ---- LDS tiles: [rows][D] bf16, 16-byte pieces XORed by the row. Eight
-// neighbouring rows spread over the eight pieces of 128 bytes (the row reads of
-// 32 lanes), and four neighbouring rows over four pairs (the transposing
-// reads): both are free of bank conflicts.
+// ---- LDS tiles: [rows][D] bf16, 16-byte pieces XORed by a function of the row.
+// LDS serves 256 bytes at a time: sixteen neighbouring rows' pieces at one
+// column (row reads), or 64 bytes of each of four neighbouring rows (the
+// transposing reads); the function sends both to 256 bytes of different banks
+// (a row of D = 64 is half of them, and which half is its lowest bit).
 template <int D>
 __device__ __forceinline__ int piece(int row, int p) {
-  const int f = ((row & 3) << 1) | ((row >> 2) & 1);
+  const int f = D == 64 ? ((row >> 1) & 1) << 2 | ((row >> 2) & 3) : (row & 3) << 2 | ((row >> 2) & 3);
   return row * 2 * D + ((p ^ f) << 4);
 }
 
@@ -79,6 +80,9 @@ __device__ __forceinline__ f16 mfma(b8 a, b8 b, f16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
 
+// one instruction of three operands, and a NaN stays
+__device__ __forceinline__ float larger(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
 __device__ __forceinline__ int crow(int r, int hi) { return (r & 3) + 8 * (r >> 2) + 4 * hi; }
 
 // C's registers 8 ks .. 8 ks + 7 as the B fragment of k-step ks
@@ -91,38 +95,66 @@ __device__ __forceinline__ b8 pack(const f16& c, int ks) {
 
 // ---- staging of 64 rows of two matrices by 256 threads, through registers so
 // that rows that must not count (masked keys, rows past the end) become zero:
-// what stands there, NaN too, cannot reach a result.
+// what stands there, NaN too, cannot reach a result. A row's place inside the
+// chunk is computed once; the chunk's start is uniform.
 template <int D>
 struct Stage {
   static constexpr int N = KC * D / 8 / 256;  // 16-byte pieces a thread, each matrix
   b8 x[N], y[N];
-  bool on[N];
+  unsigned ax[N], ay[N];  // byte offsets inside a chunk
 
   __device__ __forceinline__ static int row(int i) { return (threadIdx.x + 256 * i) / (D / 8); }
   __device__ __forceinline__ static int col(int i) { return (threadIdx.x + 256 * i) % (D / 8); }
 
-  __device__ __forceinline__ void load(const __bf16* px, long long sx, const __bf16* py, long long sy, int r0, int end) {
+  __device__ __forceinline__ void init(int sx, int sy) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int r = min(r0 + row(i), end - 1);
-      x[i] = *(const b8*)(px + r * sx + col(i) * 8);
-      y[i] = *(const b8*)(py + r * sy + col(i) * 8);
+      ax[i] = 2u * (row(i) * sx + col(i) * 8);
+      ay[i] = 2u * (row(i) * sy + col(i) * 8);
     }
   }
-  __device__ __forceinline__ void store(char* tx, char* ty) {
-    const b8 zero = {};
+  // rows r0 .. r0 + 63 of matrices with row strides sx, sy; rows from `end` on repeat the last one
+  __device__ __forceinline__ void load(const __bf16* px, int sx, const __bf16* py, int sy, int r0, int end) {
+    const char* bx = (const char*)(px + (long long)r0 * sx);
+    const char* by = (const char*)(py + (long long)r0 * sy);
+    if (r0 + KC <= end) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        x[i] = *(const b8*)(bx + ax[i]);
+        y[i] = *(const b8*)(by + ay[i]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int r = min(row(i), end - 1 - r0);
+        x[i] = *(const b8*)(bx + 2u * (r * sx + col(i) * 8));
+        y[i] = *(const b8*)(by + 2u * (r * sy + col(i) * 8));
+      }
+    }
+  }
+  __device__ __forceinline__ void store(char* tx, char* ty, unsigned long long on) {
+    if (on != ~0ull) {
+      const b8 zero = {};
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const bool keep = (on >> row(i)) & 1;
+        x[i] = keep ? x[i] : zero;
+        y[i] = keep ? y[i] : zero;
+      }
+    }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int at = piece<D>(row(i), col(i));
-      *(b8*)(tx + at) = on[i] ? x[i] : zero;
-      *(b8*)(ty + at) = on[i] ? y[i] : zero;
+      *(b8*)(tx + at) = x[i];
+      *(b8*)(ty + at) = y[i];
     }
   }
 };
 
-// ---- the bias of one head in LDS: entry x is the offset clamp(x - 3 - far),
+// ---- the bias of one head in LDS: entry x is the offset clamp(x - 7 - far),
 // copy c holds the entries from c on. `sign` -1: offsets mirrored.
-__device__ __forceinline__ int bias_len(int far) { return (2 * far + 10) & ~3; }
+__host__ __device__ __forceinline__ int bias_top(int far) { return (2 * far + 10) & ~3; }  // from here on all are the last offset's
+__host__ __device__ __forceinline__ int bias_len(int far) { return bias_top(far) + 4; }
 
 // A table value of the type's lowest stands for a mask, as -inf does: divided
 // by the scale it would leave 32 bits' range, and a sum of exponentials of it
@@ -140,7 +172,7 @@ __device__ __forceinline__ float bias_at(const RelArgs& a, int d, int h) {
 __device__ void stage_bias(const RelArgs& a, int h, int sign, float* bias) {
   const int len = bias_len(a.far);
   for (int x = threadIdx.x; x < len + 3; x += 256) {
-    const int d = min(max(x - 3 - a.far, -a.far), a.far);
+    const int d = min(max(x - 7 - a.far, -a.far), a.far);
     const float v = bias_at(a, sign * d, h);
 #pragma unroll
     for (int c = 0; c < 4; ++c)
@@ -158,12 +190,12 @@ __device__ __forceinline__ f16 bias_tile(const float* bias, int far, int row0, i
     for (int r = 0; r < 16; ++r) c[r] = v;
     return c;
   }
-  const int len = bias_len(far);
-  const int d = row0 + 4 * (lane >> 5) - (col0 + (lane & 31));
+  // which copy is the lane's own, since tiles start on multiples of 32
+  const int x = row0 + 4 * (lane >> 5) - (col0 + (lane & 31)) + far + 7, copy = x & 3;
+  const float* mine = bias + copy * bias_len(far);
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
-    const int x = min(max(d + 8 * g, -far - 3), far) + far + 3;
-    const f4 v = *(const f4*)(bias + (x & 3) * len + (x & ~3));
+    const f4 v = *(const f4*)(mine + min(max((x & ~3) + 8 * g, 0), bias_top(far)));
 #pragma unroll
     for (int e = 0; e < 4; ++e) c[4 * g + e] = v[e];
   }
@@ -226,7 +258,7 @@ __device__ __forceinline__ void store_columns(__bf16* row, const f16* c, float m
 
 // ---------------- forward: a wave owns 32 queries, chunks of 64 keys ----------------
 template <int D>
-__global__ __launch_bounds__(256) void k_rel_fwd(RelArgs a, int tiles) {
+__global__ __launch_bounds__(256, 2) void k_rel_fwd(RelArgs a, int tiles) {
   extern __shared__ __align__(16) char smem[];
   __shared__ int ends[4];
   char* buf = smem;  // [2][K, V]
@@ -238,8 +270,8 @@ __global__ __launch_bounds__(256) void k_rel_fwd(RelArgs a, int tiles) {
   const int tile = a.causal ? tiles - 1 - id % tiles : id % tiles;
   const int lane = threadIdx.x & 63, hi = lane >> 5;
   const int i0 = tile * TILE + (threadIdx.x >> 6) * 32, i = i0 + (lane & 31);
-  const __bf16* k = a.k + b * a.k_b + hk * a.k_h;
-  const __bf16* v = a.v + b * a.v_b + hk * a.v_h;
+  const __bf16* k = a.qkv + (long long)b * a.S * a.width + (a.NH + hk) * D;
+  const __bf16* v = k + a.NKV * D;
   const unsigned char* mask = a.mask ? a.mask + (long long)b * a.S : nullptr;
 
   stage_bias(a, h, 1, bias);
@@ -248,7 +280,7 @@ __global__ __launch_bounds__(256) void k_rel_fwd(RelArgs a, int tiles) {
   const int chunks = (end + KC - 1) / KC;
 
   b8 q[D / 16];
-  const __bf16* qp = a.q + b * a.q_b + min(i, a.S - 1) * a.q_s + h * a.q_h;
+  const __bf16* qp = a.qkv + ((long long)b * a.S + min(i, a.S - 1)) * a.width + h * D;
 #pragma unroll
   for (int t = 0; t < D / 16; ++t) q[t] = *(const b8*)(qp + 16 * t + 8 * hi);
 
@@ -257,19 +289,18 @@ __global__ __launch_bounds__(256) void k_rel_fwd(RelArgs a, int tiles) {
   const float c2 = a.scale * LOG2E;
 
   Stage<D> st;
+  st.init(a.width, a.width);
   unsigned long long bits = 0, next = 0;
   auto fetch = [&](int c) {
-    st.load(k, a.k_s, v, a.v_s, c * KC, end);
+    st.load(k, a.width, v, a.width, c * KC, end);
     next = key_bits(mask, c * KC, end);
-#pragma unroll
-    for (int n = 0; n < Stage<D>::N; ++n) st.on[n] = (next >> Stage<D>::row(n)) & 1;
   };
   if (chunks > 0) {
     fetch(0);
-    st.store(buf, buf + MAT);
+    st.store(buf, buf + MAT, next);
   }
   __syncthreads();
-  const float low = bias[0], high = bias[2 * a.far + 3];
+  const float low = bias[0], high = bias[2 * a.far + 7];
 
   for (int c = 0; c < chunks; ++c) {
     bits = next;
@@ -277,24 +308,29 @@ __global__ __launch_bounds__(256) void k_rel_fwd(RelArgs a, int tiles) {
     if (c > 0) __syncthreads();
     const char* kt = buf + (c & 1) * 2 * MAT;
     const char* vt = kt + MAT;
+    const int j0 = c * KC;
+    if (bits != 0 && !(a.causal && j0 > i0 + 31)) {
+      f16 s[2];
 #pragma unroll
-    for (int sub = 0; sub < 2; ++sub) {
-      const int j0 = c * KC + 32 * sub;
-      const unsigned on = (unsigned)(bits >> (32 * sub));
-      if (on == 0 || (a.causal && j0 > i0 + 31)) continue;
-      f16 s = bias_tile(bias, a.far, j0, i0, lane, low, high);
+      for (int sub = 0; sub < 2; ++sub) s[sub] = bias_tile(bias, a.far, j0 + 32 * sub, i0, lane, low, high);
 #pragma unroll
-      for (int t = 0; t < D / 16; ++t) s = mfma(row_frag<D>(kt, 32 * sub + (lane & 31), t, hi), q[t], s);
-      drop_rows(s, on, a.causal && j0 + 31 > i0, j0, i0, lane, -INF);
-      float top = s[0];
+      for (int t = 0; t < D / 16; ++t)
 #pragma unroll
-      for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
-      top = fmaxf(top, __shfl_xor(top, 32, 64)) * c2;
+        for (int sub = 0; sub < 2; ++sub) s[sub] = mfma(row_frag<D>(kt, 32 * sub + (lane & 31), t, hi), q[t], s[sub]);
+      if (bits != ~0ull || (a.causal && j0 + 63 > i0))
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub)
+          drop_rows(s[sub], (unsigned)(bits >> (32 * sub)), a.causal && j0 + 32 * sub + 31 > i0, j0 + 32 * sub, i0, lane, -INF);
+      float top = larger(s[0][0], s[1][0]);
+#pragma unroll
+      for (int r = 1; r < 16; ++r) top = larger(larger(top, s[0][r]), s[1][r]);
+      top *= c2;
       // the maximum moves only where it grew by more than 8 (a factor of 256,
       // far inside 32 bits and the same relative rounding in bf16): after the
-      // first chunks the accumulators are hardly ever rescaled
+      // first chunks the accumulators are hardly ever rescaled, and the two
+      // halves of the wave compare their maxima only then
       if (__any(top > m + 8.f)) {
-        const float n = fmaxf(m, top);
+        const float n = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64)));
         const float f = n == -INF ? 1.f : __builtin_amdgcn_exp2f(m - n);
         m = n;
         l *= f;
@@ -304,23 +340,26 @@ __global__ __launch_bounds__(256) void k_rel_fwd(RelArgs a, int tiles) {
           for (int r = 0; r < 16; ++r) o[dt][r] *= f;
       }
       const float base = m == -INF ? 0.f : m;
-      float sum = 0.f;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c2, -base));
-        sum += s[r];
-      }
-      l += sum;
+      for (int sub = 0; sub < 2; ++sub) {
+        float sum = 0.f;
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        const b8 p = pack(s, ks);
+        for (int r = 0; r < 16; ++r) {
+          s[sub][r] = __builtin_amdgcn_exp2f(fmaf(s[sub][r], c2, -base));
+          sum += s[sub][r];
+        }
+        l += sum;
 #pragma unroll
-        for (int dt = 0; dt < D / 32; ++dt) o[dt] = mfma(col_frag<D>(vt, 32 * sub + 16 * ks, dt, lane), p, o[dt]);
+        for (int ks = 0; ks < 2; ++ks) {
+          const b8 p = pack(s[sub], ks);
+#pragma unroll
+          for (int dt = 0; dt < D / 32; ++dt) o[dt] = mfma(col_frag<D>(vt, 32 * sub + 16 * ks, dt, lane), p, o[dt]);
+        }
       }
     }
     if (c + 1 < chunks) {
       char* to = buf + ((c + 1) & 1) * 2 * MAT;
-      st.store(to, to + MAT);
+      st.store(to, to + MAT, next);
     }
   }
   l += __shfl_xor(l, 32, 64);
@@ -352,7 +391,7 @@ __device__ __forceinline__ void diagonals(const f16& c, float* d) {
 
 // ---------------- backward 1: dQ, D and the offsets' sums of dS ----------------
 template <int D>
-__global__ __launch_bounds__(256) void k_rel_bwd_q(RelArgs a, int tiles) {
+__global__ __launch_bounds__(256, 2) void k_rel_bwd_q(RelArgs a, int tiles) {
   extern __shared__ __align__(16) char smem[];
   __shared__ int ends[4];
   char* buf = smem;  // [2][K, V]
@@ -366,8 +405,8 @@ __global__ __launch_bounds__(256) void k_rel_bwd_q(RelArgs a, int tiles) {
   const int tile = a.causal ? tiles - 1 - id % tiles : id % tiles;
   const int lane = threadIdx.x & 63, hi = lane >> 5, wave = threadIdx.x >> 6;
   const int i0 = tile * TILE + wave * 32, i = i0 + (lane & 31);
-  const __bf16* k = a.k + b * a.k_b + hk * a.k_h;
-  const __bf16* v = a.v + b * a.v_b + hk * a.v_h;
+  const __bf16* k = a.qkv + (long long)b * a.S * a.width + (a.NH + hk) * D;
+  const __bf16* v = k + a.NKV * D;
   const unsigned char* mask = a.mask ? a.mask + (long long)b * a.S : nullptr;
 
   stage_bias(a, h, 1, bias);
@@ -383,7 +422,7 @@ __global__ __launch_bounds__(256) void k_rel_bwd_q(RelArgs a, int tiles) {
   float dsum = 0.f;
   {
     const int r = min(i, a.S - 1);
-    const __bf16* qp = a.q + b * a.q_b + r * a.q_s + h * a.q_h;
+    const __bf16* qp = a.qkv + ((long long)b * a.S + r) * a.width + h * D;
     const long long at = (((long long)b * a.S + r) * a.NH + h) * D;
     const b8 zero = {};
 #pragma unroll
@@ -413,19 +452,18 @@ __global__ __launch_bounds__(256) void k_rel_bwd_q(RelArgs a, int tiles) {
   };
 
   Stage<D> st;
+  st.init(a.width, a.width);
   unsigned long long bits = 0, next = 0;
   auto fetch = [&](int c) {
-    st.load(k, a.k_s, v, a.v_s, c * KC, end);
+    st.load(k, a.width, v, a.width, c * KC, end);
     next = key_bits(mask, c * KC, end);
-#pragma unroll
-    for (int n = 0; n < Stage<D>::N; ++n) st.on[n] = (next >> Stage<D>::row(n)) & 1;
   };
   if (chunks > 0) {
     fetch(0);
-    st.store(buf, buf + MAT);
+    st.store(buf, buf + MAT, next);
   }
   __syncthreads();
-  const float low = bias[0], high = bias[2 * a.far + 3];
+  const float low = bias[0], high = bias[2 * a.far + 7];
 
   for (int c = 0; c < chunks; ++c) {
     bits = next;
@@ -479,11 +517,11 @@ __global__ __launch_bounds__(256) void k_rel_bwd_q(RelArgs a, int tiles) {
     }
     if (c + 1 < chunks) {
       char* to = buf + ((c + 1) & 1) * 2 * MAT;
-      st.store(to, to + MAT);
+      st.store(to, to + MAT, next);
     }
   }
   if (i < a.S)
-    store_columns<D>(a.dq + b * a.dq_b + i * a.dq_s + (long long)h * D, dq, a.scale, hi);
+    store_columns<D>(a.dqkv + ((long long)b * a.S + i) * a.width + h * D, dq, a.scale, hi);
   add(left_at - i0 + lane_off, left);
 #pragma unroll
   for (int x = 32; x > 0; x >>= 1) {
@@ -506,7 +544,7 @@ __global__ __launch_bounds__(256) void k_rel_bwd_q(RelArgs a, int tiles) {
 
 // ---------------- backward 2: dK and dV; a wave owns 32 keys, chunks of 64 queries ----------------
 template <int D>
-__global__ __launch_bounds__(256) void k_rel_bwd_kv(RelArgs a, int tiles) {
+__global__ __launch_bounds__(256, D == 64 ? 2 : 1) void k_rel_bwd_kv(RelArgs a, int tiles) {
   extern __shared__ __align__(16) char smem[];
   char* buf = smem;  // [2][Q, dO]
   constexpr int MAT = KC * 2 * D;
@@ -524,8 +562,8 @@ __global__ __launch_bounds__(256) void k_rel_bwd_kv(RelArgs a, int tiles) {
   b8 k[D / 16], v[D / 16];
   {
     const int r = min(j, a.S - 1);
-    const __bf16* kp = a.k + b * a.k_b + r * a.k_s + hk * a.k_h;
-    const __bf16* vp = a.v + b * a.v_b + r * a.v_s + hk * a.v_h;
+    const __bf16* kp = a.qkv + ((long long)b * a.S + r) * a.width + (a.NH + hk) * D;
+    const __bf16* vp = kp + a.NKV * D;
     const b8 zero = {};
 #pragma unroll
     for (int t = 0; t < D / 16; ++t) {
@@ -539,33 +577,27 @@ __global__ __launch_bounds__(256) void k_rel_bwd_kv(RelArgs a, int tiles) {
   const float c2 = a.scale * LOG2E;
   const int first = a.causal ? tile * TILE / KC : 0, chunks = (a.S + KC - 1) / KC;
   Stage<D> st;
+  st.init(a.width, a.NH * D);
   float row_lse = 0.f, row_d = 0.f;
+  unsigned long long on = 0;
 
   if (__syncthreads_or(work))
     for (int n = 0; n < group; ++n) {
       const int h = hk * group + n, bh = b * a.NH + h;
-      const __bf16* q = a.q + b * a.q_b + h * a.q_h;
+      const __bf16* q = a.qkv + (long long)b * a.S * a.width + h * D;
       const __bf16* g = a.dout + ((long long)b * a.S * a.NH + h) * D;
-      const long long g_s = (long long)a.NH * D;
       const float* lse = a.lse + (long long)bh * a.S;
       const float* dsum = a.dsum + (long long)bh * a.S;
       auto fetch = [&](int c) {
-        st.load(q, a.q_s, g, g_s, c * KC, a.S);
-#pragma unroll
-        for (int x = 0; x < Stage<D>::N; ++x) {
-          const int r = c * KC + Stage<D>::row(x);
-          const float e = r < a.S ? lse[r] : INF;
-          st.on[x] = e < INF || e != e;  // rows past the end or with nothing allowed: zeros
-        }
-        if (threadIdx.x < KC) {
-          const int r = c * KC + threadIdx.x;
-          row_lse = r < a.S ? lse[r] : INF;
-          row_d = r < a.S ? dsum[r] : 0.f;
-        }
+        st.load(q, a.width, g, a.NH * D, c * KC, a.S);
+        const int r = c * KC + lane;
+        row_lse = r < a.S ? lse[r] : INF;
+        row_d = r < a.S ? dsum[r] : 0.f;
+        on = __ballot(row_lse < INF || row_lse != row_lse);  // others: past the end, or with nothing allowed
       };
       auto put = [&](int c) {
         char* to = buf + (c & 1) * 2 * MAT;
-        st.store(to, to + MAT);
+        st.store(to, to + MAT, on);
         if (threadIdx.x < KC) {
           float* r = rows + (c & 1) * 2 * KC;
           r[threadIdx.x] = row_lse;
@@ -577,7 +609,7 @@ __global__ __launch_bounds__(256) void k_rel_bwd_kv(RelArgs a, int tiles) {
       fetch(first);
       put(first);
       __syncthreads();
-      const float low = bias[0], high = bias[2 * a.far + 3];
+      const float low = bias[0], high = bias[2 * a.far + 7];
       for (int c = first; c < chunks; ++c) {
         if (c + 1 < chunks) fetch(c + 1);
         if (c > first) __syncthreads();
@@ -631,9 +663,9 @@ __global__ __launch_bounds__(256) void k_rel_bwd_kv(RelArgs a, int tiles) {
   if (j >= a.S) return;
   // a masked key's column holds what its zeroed K and V gave: it has no gradient
   const f16 none[D / 32] = {};
-  const long long at = b * a.dk_b + j * a.dk_s + (long long)hk * D;
-  store_columns<D>(a.dk + at, keep ? dk : none, a.scale, hi);
-  store_columns<D>(a.dv + at, keep ? dv : none, 1.f, hi);
+  __bf16* at = a.dqkv + ((long long)b * a.S + j) * a.width + (a.NH + hk) * D;
+  store_columns<D>(at, keep ? dk : none, a.scale, hi);
+  store_columns<D>(at + a.NKV * D, keep ? dv : none, 1.f, hi);
 }
 
 // dtable[n][h]: the offsets' sums over batches and tiles, then over the offsets
@@ -857,7 +889,7 @@ __global__ __launch_bounds__(D) void k_rel_join(RelTokenArgs a, int row_tiles) {
       (__bf16)(z == 0.f ? 0.f : o / z);
 }
 
-size_t bias_bytes(int far) { return 16 * (size_t)((2 * far + 10) & ~3); }
+size_t bias_bytes(int far) { return 16 * (size_t)bias_len(far); }
 
 // dynamic LDS above 64 KB has to be asked for
 template <typename F>

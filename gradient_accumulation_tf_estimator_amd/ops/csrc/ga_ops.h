@@ -60,10 +60,12 @@ struct RelArgs {
   __bf16* dqkv;               // like qkv
   float* doff;                // [B * NH * tiles][2 * far + 1], tiles = rel_tiles(S)
   __bf16* dtable;             // [buckets][NH]
-  int B, S, NH, NKV, D, width, buckets, far, causal;
+  float* dkv;                 // [parts][B][NKV][S][dK, dV] where parts > 1
+  int B, S, NH, NKV, D, width, buckets, far, causal, parts;
   float scale;
 };
 int rel_tiles(int S);
+int rel_parts(int B, int S, int NH, int NKV);
 hipError_t rel_forward(const RelArgs& a, hipStream_t s);
 hipError_t rel_backward(const RelArgs& a, hipStream_t s);
 

@@ -264,7 +264,7 @@ RelArgs rel_args(const at::Tensor& qkv, int64_t NH, int64_t NKV, const at::Tenso
   TORCH_CHECK(scale > 0 && std::isfinite(scale), "scale must be positive and finite");
   // a chunk of 64 rows is addressed by 32 bits from its start
   TORCH_CHECK(qkv.size(2) <= (1 << 23), "too many heads");
-  TORCH_CHECK(S < (1ll << 24) && B * NH * (S / 128 + 1) < (1ll << 31), "too many rows");
+  TORCH_CHECK(S < (1ll << 24) && B * NH * (S / 128 + 1) < (1ll << 31) && B * NKV * S * D < (1ll << 38), "too many rows");
   if (mask)
     TORCH_CHECK(mask->device() == qkv.device() && mask->scalar_type() == at::kByte && mask->is_contiguous() &&
                 mask->dim() == 2 && mask->size(0) == B && mask->size(1) == S, "mask must be a contiguous u8 [B, S] tensor");
@@ -320,6 +320,12 @@ std::vector<at::Tensor> rel_attn_bwd(at::Tensor dout, at::Tensor qkv, at::Tensor
   }
   auto dsum = at::empty_like(lse);
   auto doff = at::empty({(int64_t)a.B * NH * rel_tiles(a.S), 2 * a.far + 1}, lse.options());
+  a.parts = rel_parts(a.B, a.S, a.NH, a.NKV);
+  at::Tensor dkv;
+  if (a.parts > 1) {
+    dkv = at::empty({(int64_t)a.parts * a.B * NKV * a.S, 2 * a.D}, lse.options());
+    a.dkv = dkv.data_ptr<float>();
+  }
   a.out = (__bf16*)out.data_ptr();
   a.lse = lse.data_ptr<float>();
   a.dout = (const __bf16*)dout.data_ptr();

@@ -243,16 +243,17 @@ __device__ __forceinline__ void drop_rows(f16& c, unsigned bits, bool diag, int 
   }
 }
 
-template <int D>
-__device__ __forceinline__ void store_columns(__bf16* row, const f16* c, float mul, int hi) {
+template <int D, typename E>
+__device__ __forceinline__ void store_columns(E* row, const f16* c, float mul, int hi) {
+  typedef __attribute__((ext_vector_type(4))) E e4;
 #pragma unroll
   for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      b4 v;
+      e4 v;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = (__bf16)(c[dt][4 * g + e] * mul);
-      *(b4*)(row + 32 * dt + 8 * g + 4 * hi) = v;
+      for (int e = 0; e < 4; ++e) v[e] = (E)(c[dt][4 * g + e] * mul);
+      *(e4*)(row + 32 * dt + 8 * g + 4 * hi) = v;
     }
 }
 
@@ -552,8 +553,8 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void k_rel_bwd_kv(RelArgs a, 
   float* bias = rows + 4 * KC;
 
   const int id = remap(blockIdx.x, gridDim.x);
-  const int bk = id / tiles, hk = bk % a.NKV, b = bk / a.NKV, group = a.NH / a.NKV;
-  const int tile = id % tiles;
+  const int tile = id % tiles, part = id / tiles % a.parts, bk = id / tiles / a.parts;
+  const int hk = bk % a.NKV, b = bk / a.NKV, group = a.NH / a.NKV;
   const int lane = threadIdx.x & 63, hi = lane >> 5;
   const int j0 = tile * TILE + (threadIdx.x >> 6) * 32, j = j0 + (lane & 31);
   const bool keep = j < a.S && (!a.mask || a.mask[(long long)b * a.S + min(j, a.S - 1)]);
@@ -582,7 +583,7 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void k_rel_bwd_kv(RelArgs a, 
   unsigned long long on = 0;
 
   if (__syncthreads_or(work))
-    for (int n = 0; n < group; ++n) {
+    for (int n = part; n < group; n += a.parts) {
       const int h = hk * group + n, bh = b * a.NH + h;
       const __bf16* q = a.qkv + (long long)b * a.S * a.width + h * D;
       const __bf16* g = a.dout + ((long long)b * a.S * a.NH + h) * D;
@@ -616,19 +617,28 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void k_rel_bwd_kv(RelArgs a, 
         const char* qt = buf + (c & 1) * 2 * MAT;
         const char* gt = qt + MAT;
         const float* rl = rows + (c & 1) * 2 * KC;
-        if (work)
+        const int i0 = c * KC;
+        if (work && !(a.causal && i0 + 63 < j0)) {
+          // rows are queries here: the mirrored bias of row - column
+          f16 s[2], dp[2] = {};
 #pragma unroll
-          for (int sub = 0; sub < 2; ++sub) {
-            const int i0 = c * KC + 32 * sub;
-            if (i0 >= a.S || (a.causal && i0 + 31 < j0)) continue;
-            // rows are queries here: the mirrored bias of row - column
-            f16 s = bias_tile(bias, a.far, i0, j0, lane, low, high);
-            f16 dp = {};
+          for (int sub = 0; sub < 2; ++sub) s[sub] = bias_tile(bias, a.far, i0 + 32 * sub, j0, lane, low, high);
+#pragma unroll
+          for (int sub = 0; sub < 2; ++sub)
 #pragma unroll
             for (int t = 0; t < D / 16; ++t) {
-              s = mfma(row_frag<D>(qt, 32 * sub + (lane & 31), t, hi), k[t], s);
-              dp = mfma(row_frag<D>(gt, 32 * sub + (lane & 31), t, hi), v[t], dp);
+              s[sub] = mfma(row_frag<D>(qt, 32 * sub + (lane & 31), t, hi), k[t], s[sub]);
+              dp[sub] = mfma(row_frag<D>(gt, 32 * sub + (lane & 31), t, hi), v[t], dp[sub]);
             }
+          if (a.causal && i0 < j0 + 31)
+#pragma unroll
+            for (int sub = 0; sub < 2; ++sub) {
+              const int least = j - i0 - 32 * sub - 4 * hi;
+#pragma unroll
+              for (int r = 0; r < 16; ++r) s[sub][r] = crow(r, 0) >= least ? s[sub][r] : -INF;
+            }
+#pragma unroll
+          for (int sub = 0; sub < 2; ++sub) {
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
               const f4 e = *(const f4*)(rl + 32 * sub + 8 * x + 4 * hi);
@@ -636,20 +646,13 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void k_rel_bwd_kv(RelArgs a, 
 #pragma unroll
               for (int y = 0; y < 4; ++y) {
                 const int r = 4 * x + y;
-                s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c2, -e[y]));
-                dp[r] = dp[r] - d[y];
+                s[sub][r] = __builtin_amdgcn_exp2f(fmaf(s[sub][r], c2, -e[y]));
+                dp[sub][r] = (dp[sub][r] - d[y]) * s[sub][r];
               }
             }
-            if (a.causal && i0 < j0 + 31) {
-              const int least = j - i0 - 4 * hi;
-#pragma unroll
-              for (int r = 0; r < 16; ++r) s[r] = crow(r, 0) >= least ? s[r] : 0.f;
-            }
-#pragma unroll
-            for (int r = 0; r < 16; ++r) dp[r] *= s[r];
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks) {
-              const b8 p = pack(s, ks), ds = pack(dp, ks);
+              const b8 p = pack(s[sub], ks), ds = pack(dp[sub], ks);
 #pragma unroll
               for (int dt = 0; dt < D / 32; ++dt) {
                 dv[dt] = mfma(col_frag<D>(gt, 32 * sub + 16 * ks, dt, lane), p, dv[dt]);
@@ -657,15 +660,40 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void k_rel_bwd_kv(RelArgs a, 
               }
             }
           }
+        }
         if (c + 1 < chunks) put(c + 1);
       }
     }
   if (j >= a.S) return;
   // a masked key's column holds what its zeroed K and V gave: it has no gradient
   const f16 none[D / 32] = {};
+  if (a.parts > 1) {
+    float* at = a.dkv + (((long long)part * a.B * a.NKV + bk) * a.S + j) * 2 * D;
+    store_columns<D>(at, keep ? dk : none, a.scale, hi);
+    store_columns<D>(at + D, keep ? dv : none, 1.f, hi);
+    return;
+  }
   __bf16* at = a.dqkv + ((long long)b * a.S + j) * a.width + (a.NH + hk) * D;
   store_columns<D>(at, keep ? dk : none, a.scale, hi);
   store_columns<D>(at + a.NKV * D, keep ? dv : none, 1.f, hi);
+}
+
+// the parts' dK and dV, added in order: four columns a thread
+__global__ __launch_bounds__(256) void k_rel_dkv(RelArgs a, long long n) {
+  const long long x = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (x >= n) return;
+  const int per = a.D / 2, c = (int)(x % per) * 4;  // of [dK, dV], 2 D columns
+  const long long row = x / per, part = (long long)a.B * a.NKV * a.S * 2 * a.D;
+  const float* p = a.dkv + row * 2 * a.D + c;
+  f4 t = *(const f4*)p;
+  for (int i = 1; i < a.parts; ++i) t += *(const f4*)(p + i * part);
+  b4 v;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = (__bf16)t[e];
+  const int s = (int)(row % a.S), hk = (int)(row / a.S % a.NKV);
+  const long long b = row / a.S / a.NKV;
+  const int head = c < a.D ? a.NH + hk : a.NH + a.NKV + hk;
+  *(b4*)(a.dqkv + (b * a.S + s) * a.width + head * a.D + c % a.D) = v;
 }
 
 // dtable[n][h]: the offsets' sums over batches and tiles, then over the offsets
@@ -918,8 +946,13 @@ hipError_t backward(const RelArgs& a, hipStream_t s) {
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL((k_rel_bwd_q<D>), dim3(a.B * a.NH * tiles), dim3(256), lds_q, s, a, tiles);
   if ((e = hipGetLastError()) != hipSuccess) return e;
-  hipLaunchKernelGGL((k_rel_bwd_kv<D>), dim3(a.B * a.NKV * tiles), dim3(256), lds_kv, s, a, tiles);
+  hipLaunchKernelGGL((k_rel_bwd_kv<D>), dim3(a.B * a.NKV * a.parts * tiles), dim3(256), lds_kv, s, a, tiles);
   if ((e = hipGetLastError()) != hipSuccess) return e;
+  if (a.parts > 1) {
+    const long long n = (long long)a.B * a.NKV * a.S * (D / 2);
+    hipLaunchKernelGGL(k_rel_dkv, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, a, n);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+  }
   hipLaunchKernelGGL(k_rel_dtable, dim3(a.NH), dim3(1024), 0, s, a, tiles);
   return hipGetLastError();
 }
@@ -940,6 +973,18 @@ hipError_t token(const RelTokenArgs& a, hipStream_t s) {
 }  // namespace
 
 int rel_tiles(int S) { return (S + TILE - 1) / TILE; }
+
+// Over how many workgroups the query heads that share a key/value head are
+// spread in the backward: one workgroup walks all queries of its heads, so
+// with few of them (and uneven ones, under the causal mask) the chip waits for
+// the longest.
+int rel_parts(int B, int S, int NH, int NKV) {
+  const int group = NH / NKV, tiles = rel_tiles(S);
+  int n = 1;
+  while (n < group && (long long)B * NKV * tiles * n < 1024) ++n;
+  while (group % n) ++n;
+  return n;
+}
 
 // enough workgroups to fill the chip twice, but at least 128 keys a wave
 int rel_token_splits(int B, int Sq, int S, int NH, int NKV) {

@@ -40,6 +40,7 @@ typedef __attribute__((ext_vector_type(8))) short s8;
 typedef __attribute__((ext_vector_type(4))) float f4;
 typedef __attribute__((ext_vector_type(16))) float f16;
 typedef __attribute__((address_space(3))) s4 lds_s4;
+typedef __attribute__((address_space(3))) char lds_char;
 
 #define LOG2E 1.44269504088896340736f
 #define INF __builtin_inff()
@@ -76,6 +77,19 @@ __device__ __forceinline__ b8 col_frag(const char* tile, int row, int dt, int la
   return __builtin_bit_cast(b8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
+// order of the instructions around: four LDS reads, then one for each matrix
+// instruction, so that a read's latency lies behind the products before it
+template <int N>
+__device__ __forceinline__ void reads_ahead() {
+  __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+  for (int i = 0; i < N - 4; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+}
+
 __device__ __forceinline__ f16 mfma(b8 a, b8 b, f16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
@@ -93,60 +107,69 @@ __device__ __forceinline__ b8 pack(const f16& c, int ks) {
   return v;
 }
 
-// ---- staging of 64 rows of two matrices by 256 threads, through registers so
-// that rows that must not count (masked keys, rows past the end) become zero:
-// what stands there, NaN too, cannot reach a result. A row's place inside the
-// chunk is computed once; the chunk's start is uniform.
+// ---- staging of 64 rows of two matrices by 256 threads, straight from memory
+// into LDS (16 bytes a lane, a wave's 1 KB side by side), so that no register
+// waits for a load: the next chunk arrives while this one is computed. The
+// tile's order is made by the addresses that the lanes read. Issued by inline
+// assembly, because behind the builtin the compiler waits for the data before
+// any LDS read that follows; nothing else in these kernels uses m0, and the
+// instruction has no register result. After `wait`, `clear` zeroes the rows
+// that must not count (masked keys, rows past the end): what stands there, NaN
+// too, cannot reach a result. Ordinary loads of the loop are issued before the
+// chunk's and used after `wait`, or their own wait would be for the chunk too.
 template <int D>
 struct Stage {
-  static constexpr int N = KC * D / 8 / 256;  // 16-byte pieces a thread, each matrix
-  b8 x[N], y[N];
-  unsigned ax[N], ay[N];  // byte offsets inside a chunk
+  static constexpr int N = KC * D / 8 / 256;  // pieces a thread, each matrix
+  unsigned ax[N], ay[N];                      // byte offsets inside a chunk
 
-  __device__ __forceinline__ static int row(int i) { return (threadIdx.x + 256 * i) / (D / 8); }
-  __device__ __forceinline__ static int col(int i) { return (threadIdx.x + 256 * i) % (D / 8); }
+  __device__ __forceinline__ static int place(int i) { return threadIdx.x * 16 + 4096 * i; }  // in a tile
+  __device__ __forceinline__ static int row(int i) { return place(i) / (2 * D); }
+  // the piece that lies there: piece() is its own inverse
+  __device__ __forceinline__ static int col(int i) { return (piece<D>(row(i), place(i) / 16 % (D / 8)) - row(i) * 2 * D) / 2; }
 
   __device__ __forceinline__ void init(int sx, int sy) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      ax[i] = 2u * (row(i) * sx + col(i) * 8);
-      ay[i] = 2u * (row(i) * sy + col(i) * 8);
+      ax[i] = 2u * (row(i) * sx + col(i));
+      ay[i] = 2u * (row(i) * sy + col(i));
     }
+  }
+  __device__ __forceinline__ static void move(const char* from, unsigned at, const char* to) {
+    const unsigned lds = __builtin_amdgcn_readfirstlane((unsigned)(size_t)(lds_char*)to);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(at), "s"(from) : "memory");
   }
   // rows r0 .. r0 + 63 of matrices with row strides sx, sy; rows from `end` on repeat the last one
-  __device__ __forceinline__ void load(const __bf16* px, int sx, const __bf16* py, int sy, int r0, int end) {
+  __device__ __forceinline__ void load(const __bf16* px, int sx, const __bf16* py, int sy, int r0, int end, char* tx, char* ty) {
     const char* bx = (const char*)(px + (long long)r0 * sx);
     const char* by = (const char*)(py + (long long)r0 * sy);
-    if (r0 + KC <= end) {
+    const int wave = (threadIdx.x >> 6) * 1024;
+    const bool whole = r0 + KC <= end;
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        x[i] = *(const b8*)(bx + ax[i]);
-        y[i] = *(const b8*)(by + ay[i]);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
+    for (int i = 0; i < N; ++i) {
+      unsigned x = ax[i], y = ay[i];
+      if (!whole) {
         const int r = min(row(i), end - 1 - r0);
-        x[i] = *(const b8*)(bx + 2u * (r * sx + col(i) * 8));
-        y[i] = *(const b8*)(by + 2u * (r * sy + col(i) * 8));
+        x = 2u * (r * sx + col(i));
+        y = 2u * (r * sy + col(i));
       }
+      move(bx, x, tx + wave + 4096 * i);
+      move(by, y, ty + wave + 4096 * i);
     }
   }
-  __device__ __forceinline__ void store(char* tx, char* ty, unsigned long long on) {
+  __device__ __forceinline__ static void wait() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0); the compiler knows it, and waits for no earlier load again
+    asm volatile("" ::: "memory");
+  }
+  __device__ __forceinline__ void clear(char* tx, char* ty, unsigned long long on) {
     if (on != ~0ull) {
       const b8 zero = {};
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const bool keep = (on >> row(i)) & 1;
-        x[i] = keep ? x[i] : zero;
-        y[i] = keep ? y[i] : zero;
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int at = piece<D>(row(i), col(i));
-      *(b8*)(tx + at) = x[i];
-      *(b8*)(ty + at) = y[i];
+      for (int i = 0; i < N; ++i)
+        if (!((on >> row(i)) & 1)) {
+          *(b8*)(tx + place(i)) = zero;
+          *(b8*)(ty + place(i)) = zero;
+        }
     }
   }
 };
@@ -221,11 +244,10 @@ __device__ int mask_end(const unsigned char* mask, int end, int* lds) {
   return last;
 }
 
-// which of a chunk's 64 keys count, one bit each
-__device__ __forceinline__ unsigned long long key_bits(const unsigned char* mask, int j0, int end) {
+// whether this lane's key of a chunk of 64 counts
+__device__ __forceinline__ bool key_on(const unsigned char* mask, int j0, int end) {
   const int j = j0 + (threadIdx.x & 63);
-  const bool on = j < end && (!mask || mask[min(j, end - 1)]);
-  return __ballot(on);
+  return j < end && (!mask || mask[min(j, end - 1)]);
 }
 
 // C rows whose key does not count, or lies behind the column's query -> fill
@@ -260,11 +282,11 @@ __device__ __forceinline__ void store_columns(E* row, const f16* c, float mul, i
 // ---------------- forward: a wave owns 32 queries, chunks of 64 keys ----------------
 template <int D>
 __global__ __launch_bounds__(256, 2) void k_rel_fwd(RelArgs a, int tiles) {
-  extern __shared__ __align__(16) char smem[];
-  __shared__ int ends[4];
+  extern __shared__ __align__(16) char smem[];  // the tiles lie in the first 64 KB, which m0 reaches
   char* buf = smem;  // [2][K, V]
   constexpr int MAT = KC * 2 * D;
   float* bias = (float*)(smem + 4 * MAT);
+  int* ends = (int*)(bias + 4 * bias_len(a.far));
 
   const int id = remap(blockIdx.x, gridDim.x);
   const int bh = id / tiles, h = bh % a.NH, b = bh / a.NH, hk = h / (a.NH / a.NKV);
@@ -292,21 +314,30 @@ __global__ __launch_bounds__(256, 2) void k_rel_fwd(RelArgs a, int tiles) {
   Stage<D> st;
   st.init(a.width, a.width);
   unsigned long long bits = 0, next = 0;
+  bool key = false;
   auto fetch = [&](int c) {
-    st.load(k, a.width, v, a.width, c * KC, end);
-    next = key_bits(mask, c * KC, end);
+    char* to = buf + (c & 1) * 2 * MAT;
+    key = key_on(mask, c * KC, end);
+    st.load(k, a.width, v, a.width, c * KC, end, to, to + MAT);
   };
+  auto arrive = [&](int c) {
+    char* to = buf + (c & 1) * 2 * MAT;
+    st.wait();
+    next = __ballot(key);
+    st.clear(to, to + MAT, next);
+  };
+  st.wait();
   if (chunks > 0) {
     fetch(0);
-    st.store(buf, buf + MAT, next);
+    arrive(0);
   }
   __syncthreads();
   const float low = bias[0], high = bias[2 * a.far + 7];
 
   for (int c = 0; c < chunks; ++c) {
     bits = next;
-    if (c + 1 < chunks) fetch(c + 1);
     if (c > 0) __syncthreads();
+    if (c + 1 < chunks) fetch(c + 1);
     const char* kt = buf + (c & 1) * 2 * MAT;
     const char* vt = kt + MAT;
     const int j0 = c * KC;
@@ -318,6 +349,7 @@ __global__ __launch_bounds__(256, 2) void k_rel_fwd(RelArgs a, int tiles) {
       for (int t = 0; t < D / 16; ++t)
 #pragma unroll
         for (int sub = 0; sub < 2; ++sub) s[sub] = mfma(row_frag<D>(kt, 32 * sub + (lane & 31), t, hi), q[t], s[sub]);
+      reads_ahead<D / 8>();
       if (bits != ~0ull || (a.causal && j0 + 63 > i0))
 #pragma unroll
         for (int sub = 0; sub < 2; ++sub)
@@ -358,10 +390,7 @@ __global__ __launch_bounds__(256, 2) void k_rel_fwd(RelArgs a, int tiles) {
         }
       }
     }
-    if (c + 1 < chunks) {
-      char* to = buf + ((c + 1) & 1) * 2 * MAT;
-      st.store(to, to + MAT, next);
-    }
+    if (c + 1 < chunks) arrive(c + 1);
   }
   l += __shfl_xor(l, 32, 64);
   if (i >= a.S) return;
@@ -393,13 +422,13 @@ __device__ __forceinline__ void diagonals(const f16& c, float* d) {
 // ---------------- backward 1: dQ, D and the offsets' sums of dS ----------------
 template <int D>
 __global__ __launch_bounds__(256, 2) void k_rel_bwd_q(RelArgs a, int tiles) {
-  extern __shared__ __align__(16) char smem[];
-  __shared__ int ends[4];
+  extern __shared__ __align__(16) char smem[];  // the tiles lie in the first 64 KB, which m0 reaches
   char* buf = smem;  // [2][K, V]
   constexpr int MAT = KC * 2 * D;
   float* bias = (float*)(smem + 4 * MAT);
   const int offs = 2 * a.far + 1;
-  float* sums = bias + 4 * bias_len(a.far);  // [4 waves][2 halves][offs]
+  int* ends = (int*)(bias + 4 * bias_len(a.far));
+  float* sums = (float*)(ends + 4);  // [4 waves][2 halves][offs]
 
   const int id = remap(blockIdx.x, gridDim.x);
   const int bh = id / tiles, h = bh % a.NH, b = bh / a.NH, hk = h / (a.NH / a.NKV);
@@ -455,21 +484,30 @@ __global__ __launch_bounds__(256, 2) void k_rel_bwd_q(RelArgs a, int tiles) {
   Stage<D> st;
   st.init(a.width, a.width);
   unsigned long long bits = 0, next = 0;
+  bool key = false;
   auto fetch = [&](int c) {
-    st.load(k, a.width, v, a.width, c * KC, end);
-    next = key_bits(mask, c * KC, end);
+    char* to = buf + (c & 1) * 2 * MAT;
+    key = key_on(mask, c * KC, end);
+    st.load(k, a.width, v, a.width, c * KC, end, to, to + MAT);
   };
+  auto arrive = [&](int c) {
+    char* to = buf + (c & 1) * 2 * MAT;
+    st.wait();
+    next = __ballot(key);
+    st.clear(to, to + MAT, next);
+  };
+  st.wait();
   if (chunks > 0) {
     fetch(0);
-    st.store(buf, buf + MAT, next);
+    arrive(0);
   }
   __syncthreads();
   const float low = bias[0], high = bias[2 * a.far + 7];
 
   for (int c = 0; c < chunks; ++c) {
     bits = next;
-    if (c + 1 < chunks) fetch(c + 1);
     if (c > 0) __syncthreads();
+    if (c + 1 < chunks) fetch(c + 1);
     const char* kt = buf + (c & 1) * 2 * MAT;
     const char* vt = kt + MAT;
 #pragma unroll
@@ -484,6 +522,7 @@ __global__ __launch_bounds__(256, 2) void k_rel_bwd_q(RelArgs a, int tiles) {
         s = mfma(row_frag<D>(kt, 32 * sub + (lane & 31), t, hi), q[t], s);
         dp = mfma(row_frag<D>(vt, 32 * sub + (lane & 31), t, hi), g[t], dp);
       }
+      reads_ahead<D / 8>();
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c2, -lse)) * (dp[r] - dsum);
       drop_rows(s, on, a.causal && j0 + 31 > i0, j0, i0, lane, 0.f);
@@ -516,10 +555,7 @@ __global__ __launch_bounds__(256, 2) void k_rel_bwd_q(RelArgs a, int tiles) {
         for (int dt = 0; dt < D / 32; ++dt) dq[dt] = mfma(col_frag<D>(kt, 32 * sub + 16 * ks, dt, lane), p, dq[dt]);
       }
     }
-    if (c + 1 < chunks) {
-      char* to = buf + ((c + 1) & 1) * 2 * MAT;
-      st.store(to, to + MAT, next);
-    }
+    if (c + 1 < chunks) arrive(c + 1);
   }
   if (i < a.S)
     store_columns<D>(a.dqkv + ((long long)b * a.S + i) * a.width + h * D, dq, a.scale, hi);
@@ -580,7 +616,7 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void k_rel_bwd_kv(RelArgs a, 
   Stage<D> st;
   st.init(a.width, a.NH * D);
   float row_lse = 0.f, row_d = 0.f;
-  unsigned long long on = 0;
+  st.wait();
 
   if (__syncthreads_or(work))
     for (int n = part; n < group; n += a.parts) {
@@ -590,15 +626,17 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void k_rel_bwd_kv(RelArgs a, 
       const float* lse = a.lse + (long long)bh * a.S;
       const float* dsum = a.dsum + (long long)bh * a.S;
       auto fetch = [&](int c) {
-        st.load(q, a.width, g, a.NH * D, c * KC, a.S);
+        char* to = buf + (c & 1) * 2 * MAT;
         const int r = c * KC + lane;
-        row_lse = r < a.S ? lse[r] : INF;
-        row_d = r < a.S ? dsum[r] : 0.f;
-        on = __ballot(row_lse < INF || row_lse != row_lse);  // others: past the end, or with nothing allowed
+        row_lse = lse[min(r, a.S - 1)];
+        row_d = dsum[min(r, a.S - 1)];
+        st.load(q, a.width, g, a.NH * D, c * KC, a.S, to, to + MAT);
       };
       auto put = [&](int c) {
         char* to = buf + (c & 1) * 2 * MAT;
-        st.store(to, to + MAT, on);
+        st.wait();
+        if (c * KC + lane >= a.S) row_lse = INF, row_d = 0.f;
+        st.clear(to, to + MAT, __ballot(row_lse < INF || row_lse != row_lse));  // rows with nothing allowed too
         if (threadIdx.x < KC) {
           float* r = rows + (c & 1) * 2 * KC;
           r[threadIdx.x] = row_lse;
@@ -612,52 +650,46 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void k_rel_bwd_kv(RelArgs a, 
       __syncthreads();
       const float low = bias[0], high = bias[2 * a.far + 7];
       for (int c = first; c < chunks; ++c) {
-        if (c + 1 < chunks) fetch(c + 1);
         if (c > first) __syncthreads();
+        if (c + 1 < chunks) fetch(c + 1);
         const char* qt = buf + (c & 1) * 2 * MAT;
         const char* gt = qt + MAT;
         const float* rl = rows + (c & 1) * 2 * KC;
-        const int i0 = c * KC;
-        if (work && !(a.causal && i0 + 63 < j0)) {
+#pragma unroll 1
+        for (int sub = 0; sub < 2; ++sub) {
+          const int i0 = c * KC + 32 * sub;
+          if (!work || i0 >= a.S || (a.causal && i0 + 31 < j0)) continue;
           // rows are queries here: the mirrored bias of row - column
-          f16 s[2], dp[2] = {};
+          f16 s = bias_tile(bias, a.far, i0, j0, lane, low, high), dp = {};
 #pragma unroll
-          for (int sub = 0; sub < 2; ++sub) s[sub] = bias_tile(bias, a.far, i0 + 32 * sub, j0, lane, low, high);
+          for (int t = 0; t < D / 16; ++t) {
+            s = mfma(row_frag<D>(qt + 64 * D * sub, lane & 31, t, hi), k[t], s);
+            dp = mfma(row_frag<D>(gt + 64 * D * sub, lane & 31, t, hi), v[t], dp);
+          }
+          reads_ahead<D / 8>();
+          if (a.causal && i0 < j0 + 31) {
+            const int least = j - i0 - 4 * hi;
 #pragma unroll
-          for (int sub = 0; sub < 2; ++sub)
+            for (int r = 0; r < 16; ++r) s[r] = crow(r, 0) >= least ? s[r] : -INF;
+          }
 #pragma unroll
-            for (int t = 0; t < D / 16; ++t) {
-              s[sub] = mfma(row_frag<D>(qt, 32 * sub + (lane & 31), t, hi), k[t], s[sub]);
-              dp[sub] = mfma(row_frag<D>(gt, 32 * sub + (lane & 31), t, hi), v[t], dp[sub]);
+          for (int x = 0; x < 4; ++x) {
+            const f4 e = *(const f4*)(rl + 32 * sub + 8 * x + 4 * hi);
+            const f4 d = *(const f4*)(rl + KC + 32 * sub + 8 * x + 4 * hi);
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+              const int r = 4 * x + y;
+              s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c2, -e[y]));
+              dp[r] = (dp[r] - d[y]) * s[r];
             }
-          if (a.causal && i0 < j0 + 31)
+          }
 #pragma unroll
-            for (int sub = 0; sub < 2; ++sub) {
-              const int least = j - i0 - 32 * sub - 4 * hi;
+          for (int ks = 0; ks < 2; ++ks) {
+            const b8 p = pack(s, ks), ds = pack(dp, ks);
 #pragma unroll
-              for (int r = 0; r < 16; ++r) s[sub][r] = crow(r, 0) >= least ? s[sub][r] : -INF;
-            }
-#pragma unroll
-          for (int sub = 0; sub < 2; ++sub) {
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              const f4 e = *(const f4*)(rl + 32 * sub + 8 * x + 4 * hi);
-              const f4 d = *(const f4*)(rl + KC + 32 * sub + 8 * x + 4 * hi);
-#pragma unroll
-              for (int y = 0; y < 4; ++y) {
-                const int r = 4 * x + y;
-                s[sub][r] = __builtin_amdgcn_exp2f(fmaf(s[sub][r], c2, -e[y]));
-                dp[sub][r] = (dp[sub][r] - d[y]) * s[sub][r];
-              }
-            }
-#pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
-              const b8 p = pack(s[sub], ks), ds = pack(dp[sub], ks);
-#pragma unroll
-              for (int dt = 0; dt < D / 32; ++dt) {
-                dv[dt] = mfma(col_frag<D>(gt, 32 * sub + 16 * ks, dt, lane), p, dv[dt]);
-                dk[dt] = mfma(col_frag<D>(qt, 32 * sub + 16 * ks, dt, lane), ds, dk[dt]);
-              }
+            for (int dt = 0; dt < D / 32; ++dt) {
+              dv[dt] = mfma(col_frag<D>(gt + 64 * D * sub, 16 * ks, dt, lane), p, dv[dt]);
+              dk[dt] = mfma(col_frag<D>(qt + 64 * D * sub, 16 * ks, dt, lane), ds, dk[dt]);
             }
           }
         }
@@ -929,7 +961,7 @@ hipError_t allow(F* f, size_t bytes) {
 template <int D>
 hipError_t forward(const RelArgs& a, hipStream_t s) {
   const int tiles = rel_tiles(a.S);
-  const size_t lds = 4 * KC * 2 * D + bias_bytes(a.far);
+  const size_t lds = 4 * KC * 2 * D + bias_bytes(a.far) + 16;
   const hipError_t e = allow(k_rel_fwd<D>, lds);
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL((k_rel_fwd<D>), dim3(a.B * a.NH * tiles), dim3(256), lds, s, a, tiles);
@@ -939,7 +971,7 @@ hipError_t forward(const RelArgs& a, hipStream_t s) {
 template <int D>
 hipError_t backward(const RelArgs& a, hipStream_t s) {
   const int tiles = rel_tiles(a.S);
-  const size_t lds_q = 4 * KC * 2 * D + bias_bytes(a.far) + 32 * (2 * a.far + 1);
+  const size_t lds_q = 4 * KC * 2 * D + bias_bytes(a.far) + 16 + 32 * (2 * a.far + 1);
   const size_t lds_kv = 4 * KC * 2 * D + 16 * KC + bias_bytes(a.far);
   hipError_t e = allow(k_rel_bwd_q<D>, lds_q);
   if (e == hipSuccess) e = allow(k_rel_bwd_kv<D>, lds_kv);

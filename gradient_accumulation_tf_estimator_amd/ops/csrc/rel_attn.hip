@@ -225,10 +225,32 @@ __device__ __forceinline__ f16 bias_tile(const float* bias, int far, int row0, i
   return c;
 }
 
-// the workgroup's (batch and head, tile): neighbours in one XCD's share of the
-// ids (id mod 8) work on one head, so that its K and V stay in that XCD's L2
-__device__ __forceinline__ int remap(int id, int n) {
-  return (n & 7) ? id : (id & 7) * (n >> 3) + (id >> 3);
+// Which tile of which head a workgroup works on. Workgroups go to the eight XCDs
+// by turns, and each XCD has an L2 of its own, so all tiles of the heads that
+// share keys go to one XCD; neighbouring units (a batch's key heads) go to
+// different ones, since batches differ in length. Under the causal mask tiles
+// differ in work too: of some 128 workgroups at a time the longest start first.
+// `units` share nothing with each other, `per` columns of a unit share its keys
+// (query heads, or parts of them). Returns unit * per + column.
+__device__ __forceinline__ int place(int units, int per, int tiles, bool by_work, int& tile) {
+  int xcd = 0, step = 1, at = blockIdx.x, columns = units * per;
+  if ((units & 7) == 0) {
+    xcd = at & 7;
+    at >>= 3;
+    step = 8;
+    columns >>= 3;
+  }
+  int c;
+  if (by_work) {
+    const int most = max(1, 128 / tiles), first = at / (most * tiles) * most, n = min(most, columns - first);
+    at -= first * tiles;
+    tile = at / n;
+    c = first + at % n;
+  } else {
+    tile = at % tiles;
+    c = at / tiles;
+  }
+  return (xcd + c / per * step) * per + c % per;
 }
 
 // one past the last key that the mask leaves, 0 if it leaves none. All threads.
@@ -288,9 +310,10 @@ __global__ __launch_bounds__(256, 2) void k_rel_fwd(RelArgs a, int tiles) {
   float* bias = (float*)(smem + 4 * MAT);
   int* ends = (int*)(bias + 4 * bias_len(a.far));
 
-  const int id = remap(blockIdx.x, gridDim.x);
-  const int bh = id / tiles, h = bh % a.NH, b = bh / a.NH, hk = h / (a.NH / a.NKV);
-  const int tile = a.causal ? tiles - 1 - id % tiles : id % tiles;
+  int tile;
+  const int bh = place(a.B * a.NKV, a.NH / a.NKV, tiles, a.causal, tile);
+  const int h = bh % a.NH, b = bh / a.NH, hk = h / (a.NH / a.NKV);
+  if (a.causal) tile = tiles - 1 - tile;  // the last tile has the most keys
   const int lane = threadIdx.x & 63, hi = lane >> 5;
   const int i0 = tile * TILE + (threadIdx.x >> 6) * 32, i = i0 + (lane & 31);
   const __bf16* k = a.qkv + (long long)b * a.S * a.width + (a.NH + hk) * D;
@@ -430,9 +453,10 @@ __global__ __launch_bounds__(256, 2) void k_rel_bwd_q(RelArgs a, int tiles) {
   int* ends = (int*)(bias + 4 * bias_len(a.far));
   float* sums = (float*)(ends + 4);  // [4 waves][2 halves][offs]
 
-  const int id = remap(blockIdx.x, gridDim.x);
-  const int bh = id / tiles, h = bh % a.NH, b = bh / a.NH, hk = h / (a.NH / a.NKV);
-  const int tile = a.causal ? tiles - 1 - id % tiles : id % tiles;
+  int tile;
+  const int bh = place(a.B * a.NKV, a.NH / a.NKV, tiles, a.causal, tile);
+  const int h = bh % a.NH, b = bh / a.NH, hk = h / (a.NH / a.NKV);
+  if (a.causal) tile = tiles - 1 - tile;  // the last tile has the most keys
   const int lane = threadIdx.x & 63, hi = lane >> 5, wave = threadIdx.x >> 6;
   const int i0 = tile * TILE + wave * 32, i = i0 + (lane & 31);
   const __bf16* k = a.qkv + (long long)b * a.S * a.width + (a.NH + hk) * D;
@@ -588,8 +612,9 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void k_rel_bwd_kv(RelArgs a, 
   float* rows = (float*)(smem + 4 * MAT);  // [2][lse, D][64]
   float* bias = rows + 4 * KC;
 
-  const int id = remap(blockIdx.x, gridDim.x);
-  const int tile = id % tiles, part = id / tiles % a.parts, bk = id / tiles / a.parts;
+  int tile;
+  const int column = place(a.B * a.NKV, a.parts, tiles, a.causal, tile);  // the first tile has the most queries
+  const int part = column % a.parts, bk = column / a.parts;
   const int hk = bk % a.NKV, b = bk / a.NKV, group = a.NH / a.NKV;
   const int lane = threadIdx.x & 63, hi = lane >> 5;
   const int j0 = tile * TILE + (threadIdx.x >> 6) * 32, j = j0 + (lane & 31);

@@ -58,7 +58,7 @@ struct RelArgs {
   const __bf16* dout;         // [B][S][NH][D]
   float* dsum;                // [B][NH][S]
   __bf16* dqkv;               // like qkv
-  float* doff;                // [B * NH * tiles][2 * far + 1], tiles = rel_tiles(S)
+  float* doff;                // [NH][B][tiles][2 * far + 1], tiles = rel_tiles(S)
   __bf16* dtable;             // [buckets][NH]
   float* dkv;                 // [parts][B][NKV][S][dK, dV] where parts > 1
   int B, S, NH, NKV, D, width, buckets, far, causal, parts;

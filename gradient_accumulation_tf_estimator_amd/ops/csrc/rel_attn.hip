@@ -107,7 +107,7 @@ __device__ __forceinline__ b8 pack(const f16& c, int ks) {
   return v;
 }
 
-// ---- staging of 64 rows of two matrices by 256 threads, straight from memory
+// ---- staging of 64 rows of two matrices by T threads, straight from memory
 // into LDS (16 bytes a lane, a wave's 1 KB side by side), so that no register
 // waits for a load: the next chunk arrives while this one is computed. The
 // tile's order is made by the addresses that the lanes read. Issued by inline
@@ -117,12 +117,12 @@ __device__ __forceinline__ b8 pack(const f16& c, int ks) {
 // that must not count (masked keys, rows past the end): what stands there, NaN
 // too, cannot reach a result. Ordinary loads of the loop are issued before the
 // chunk's and used after `wait`, or their own wait would be for the chunk too.
-template <int D>
+template <int D, int T = 256>
 struct Stage {
-  static constexpr int N = KC * D / 8 / 256;  // pieces a thread, each matrix
+  static constexpr int N = KC * D / 8 / T;  // pieces a thread, each matrix
   unsigned ax[N], ay[N];                      // byte offsets inside a chunk
 
-  __device__ __forceinline__ static int place(int i) { return threadIdx.x * 16 + 4096 * i; }  // in a tile
+  __device__ __forceinline__ static int place(int i) { return (threadIdx.x + T * i) * 16; }  // in a tile
   __device__ __forceinline__ static int row(int i) { return place(i) / (2 * D); }
   // the piece that lies there: piece() is its own inverse
   __device__ __forceinline__ static int col(int i) { return (piece<D>(row(i), place(i) / 16 % (D / 8)) - row(i) * 2 * D) / 2; }
@@ -152,8 +152,8 @@ struct Stage {
         x = 2u * (r * sx + col(i));
         y = 2u * (r * sy + col(i));
       }
-      move(bx, x, tx + wave + 4096 * i);
-      move(by, y, ty + wave + 4096 * i);
+      move(bx, x, tx + wave + 16 * T * i);
+      move(by, y, ty + wave + 16 * T * i);
     }
   }
   __device__ __forceinline__ static void wait() {
@@ -192,9 +192,10 @@ __device__ __forceinline__ float bias_at(const RelArgs& a, int d, int h) {
   return as_bias(a.table[(long long)n * a.NH + h], a.scale);
 }
 
+template <int T = 256>
 __device__ void stage_bias(const RelArgs& a, int h, int sign, float* bias) {
   const int len = bias_len(a.far);
-  for (int x = threadIdx.x; x < len + 3; x += 256) {
+  for (int x = threadIdx.x; x < len + 3; x += T) {
     const int d = min(max(x - 7 - a.far, -a.far), a.far);
     const float v = bias_at(a, sign * d, h);
 #pragma unroll
@@ -229,7 +230,7 @@ __device__ __forceinline__ f16 bias_tile(const float* bias, int far, int row0, i
 // by turns, and each XCD has an L2 of its own, so all tiles of the heads that
 // share keys go to one XCD; neighbouring units (a batch's key heads) go to
 // different ones, since batches differ in length. Under the causal mask tiles
-// differ in work too: of some 128 workgroups at a time the longest start first.
+// differ in work too: of some 64 workgroups at a time the longest start first.
 // `units` share nothing with each other, `per` columns of a unit share its keys
 // (query heads, or parts of them). Returns unit * per + column.
 __device__ __forceinline__ int place(int units, int per, int tiles, bool by_work, int& tile) {
@@ -242,7 +243,7 @@ __device__ __forceinline__ int place(int units, int per, int tiles, bool by_work
   }
   int c;
   if (by_work) {
-    const int most = max(1, 128 / tiles), first = at / (most * tiles) * most, n = min(most, columns - first);
+    const int most = max(1, 64 / tiles), first = at / (most * tiles) * most, n = min(most, columns - first);
     at -= first * tiles;
     tile = at / n;
     c = first + at % n;
@@ -594,7 +595,7 @@ __global__ __launch_bounds__(256, 2) void k_rel_bwd_q(RelArgs a, int tiles) {
     mine[offs - 1] += far_high;
   }
   __syncthreads();
-  float* to = a.doff + ((long long)bh * tiles + tile) * offs;
+  float* to = a.doff + (((long long)h * a.B + b) * tiles + tile) * offs;
   for (int x = threadIdx.x; x < offs; x += 256) {
     float t = 0.f;
 #pragma unroll
@@ -604,10 +605,16 @@ __global__ __launch_bounds__(256, 2) void k_rel_bwd_q(RelArgs a, int tiles) {
 }
 
 // ---------------- backward 2: dK and dV; a wave owns 32 keys, chunks of 64 queries ----------------
-template <int D>
-__global__ __launch_bounds__(256, D == 64 ? 2 : 1) void k_rel_bwd_kv(RelArgs a, int tiles) {
-  extern __shared__ __align__(16) char smem[];
-  char* buf = smem;  // [2][Q, dO]
+// SPLIT (head size 128): dK, dV, K and V of 32 keys fill a wave's registers, one
+// wave a SIMD is left, and products and exponentials wait for each other. So two
+// waves share the keys: the first four make dV, the other four dK. Both compute
+// the scores (40 matrix instructions a tile instead of 32), but two waves a SIMD
+// run side by side: MEASURED
+template <int D, bool SPLIT>
+__global__ __launch_bounds__(SPLIT ? 512 : 256, 2) void k_rel_bwd_kv(RelArgs a, int tiles) {
+  constexpr int T = SPLIT ? 512 : 256;
+  extern __shared__ __align__(16) char smem[];  // the tiles lie in the first 64 KB, which m0 reaches
+  char* buf = smem;                             // [2][Q, dO]
   constexpr int MAT = KC * 2 * D;
   float* rows = (float*)(smem + 4 * MAT);  // [2][lse, D][64]
   float* bias = rows + 4 * KC;
@@ -617,7 +624,9 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void k_rel_bwd_kv(RelArgs a, 
   const int part = column % a.parts, bk = column / a.parts;
   const int hk = bk % a.NKV, b = bk / a.NKV, group = a.NH / a.NKV;
   const int lane = threadIdx.x & 63, hi = lane >> 5;
-  const int j0 = tile * TILE + (threadIdx.x >> 6) * 32, j = j0 + (lane & 31);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const bool for_k = SPLIT && wave >= 4;
+  const int j0 = tile * TILE + (wave & 3) * 32, j = j0 + (lane & 31);
   const bool keep = j < a.S && (!a.mask || a.mask[(long long)b * a.S + min(j, a.S - 1)]);
   const bool work = __any(keep);  // this wave has a key that counts
 
@@ -635,10 +644,10 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void k_rel_bwd_kv(RelArgs a, 
       v[t] = keep ? v[t] : zero;
     }
   }
-  f16 dk[D / 32] = {}, dv[D / 32] = {};
+  f16 acc[D / 32] = {}, dv[SPLIT ? 1 : D / 32] = {};  // dK (SPLIT: dK or dV), dV
   const float c2 = a.scale * LOG2E;
   const int first = a.causal ? tile * TILE / KC : 0, chunks = (a.S + KC - 1) / KC;
-  Stage<D> st;
+  Stage<D, T> st;
   st.init(a.width, a.NH * D);
   float row_lse = 0.f, row_d = 0.f;
   st.wait();
@@ -669,7 +678,7 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void k_rel_bwd_kv(RelArgs a, 
         }
       };
       __syncthreads();  // the last head's tiles are read
-      stage_bias(a, h, -1, bias);
+      stage_bias<T>(a, h, -1, bias);
       fetch(first);
       put(first);
       __syncthreads();
@@ -684,14 +693,27 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void k_rel_bwd_kv(RelArgs a, 
         for (int sub = 0; sub < 2; ++sub) {
           const int i0 = c * KC + 32 * sub;
           if (!work || i0 >= a.S || (a.causal && i0 + 31 < j0)) continue;
+          const char* qs = qt + 64 * D * sub;
+          const char* gs = gt + 64 * D * sub;
           // rows are queries here: the mirrored bias of row - column
           f16 s = bias_tile(bias, a.far, i0, j0, lane, low, high), dp = {};
+          if (SPLIT) {
 #pragma unroll
-          for (int t = 0; t < D / 16; ++t) {
-            s = mfma(row_frag<D>(qt + 64 * D * sub, lane & 31, t, hi), k[t], s);
-            dp = mfma(row_frag<D>(gt + 64 * D * sub, lane & 31, t, hi), v[t], dp);
+            for (int t = 0; t < D / 16; ++t) s = mfma(row_frag<D>(qs, lane & 31, t, hi), k[t], s);
+            reads_ahead<D / 16>();
+            if (for_k) {
+#pragma unroll
+              for (int t = 0; t < D / 16; ++t) dp = mfma(row_frag<D>(gs, lane & 31, t, hi), v[t], dp);
+              reads_ahead<D / 16>();
+            }
+          } else {
+#pragma unroll
+            for (int t = 0; t < D / 16; ++t) {
+              s = mfma(row_frag<D>(qs, lane & 31, t, hi), k[t], s);
+              dp = mfma(row_frag<D>(gs, lane & 31, t, hi), v[t], dp);
+            }
+            reads_ahead<D / 8>();
           }
-          reads_ahead<D / 8>();
           if (a.causal && i0 < j0 + 31) {
             const int least = j - i0 - 4 * hi;
 #pragma unroll
@@ -700,21 +722,34 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void k_rel_bwd_kv(RelArgs a, 
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
             const f4 e = *(const f4*)(rl + 32 * sub + 8 * x + 4 * hi);
-            const f4 d = *(const f4*)(rl + KC + 32 * sub + 8 * x + 4 * hi);
 #pragma unroll
-            for (int y = 0; y < 4; ++y) {
-              const int r = 4 * x + y;
-              s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c2, -e[y]));
-              dp[r] = (dp[r] - d[y]) * s[r];
-            }
+            for (int y = 0; y < 4; ++y) s[4 * x + y] = __builtin_amdgcn_exp2f(fmaf(s[4 * x + y], c2, -e[y]));
           }
+          if (!SPLIT || for_k)
 #pragma unroll
-          for (int ks = 0; ks < 2; ++ks) {
-            const b8 p = pack(s, ks), ds = pack(dp, ks);
+            for (int x = 0; x < 4; ++x) {
+              const f4 d = *(const f4*)(rl + KC + 32 * sub + 8 * x + 4 * hi);
 #pragma unroll
-            for (int dt = 0; dt < D / 32; ++dt) {
-              dv[dt] = mfma(col_frag<D>(gt + 64 * D * sub, 16 * ks, dt, lane), p, dv[dt]);
-              dk[dt] = mfma(col_frag<D>(qt + 64 * D * sub, 16 * ks, dt, lane), ds, dk[dt]);
+              for (int y = 0; y < 4; ++y) dp[4 * x + y] = (dp[4 * x + y] - d[y]) * s[4 * x + y];
+            }
+          if (SPLIT) {
+            const char* from = for_k ? qs : gs;
+            if (for_k) s = dp;
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+              const b8 p = pack(s, ks);
+#pragma unroll
+              for (int dt = 0; dt < D / 32; ++dt) acc[dt] = mfma(col_frag<D>(from, 16 * ks, dt, lane), p, acc[dt]);
+            }
+          } else {
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+              const b8 p = pack(s, ks), ds = pack(dp, ks);
+#pragma unroll
+              for (int dt = 0; dt < D / 32; ++dt) {
+                dv[SPLIT ? 0 : dt] = mfma(col_frag<D>(gs, 16 * ks, dt, lane), p, dv[SPLIT ? 0 : dt]);
+                acc[dt] = mfma(col_frag<D>(qs, 16 * ks, dt, lane), ds, acc[dt]);
+              }
             }
           }
         }
@@ -724,15 +759,12 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void k_rel_bwd_kv(RelArgs a, 
   if (j >= a.S) return;
   // a masked key's column holds what its zeroed K and V gave: it has no gradient
   const f16 none[D / 32] = {};
-  if (a.parts > 1) {
-    float* at = a.dkv + (((long long)part * a.B * a.NKV + bk) * a.S + j) * 2 * D;
-    store_columns<D>(at, keep ? dk : none, a.scale, hi);
-    store_columns<D>(at + D, keep ? dv : none, 1.f, hi);
-    return;
-  }
-  __bf16* at = a.dqkv + ((long long)b * a.S + j) * a.width + (a.NH + hk) * D;
-  store_columns<D>(at, keep ? dk : none, a.scale, hi);
-  store_columns<D>(at + a.NKV * D, keep ? dv : none, 1.f, hi);
+  auto write = [&](auto* at, int step) {
+    if (!SPLIT || for_k) store_columns<D>(at, keep ? acc : none, a.scale, hi);
+    if (SPLIT ? !for_k : true) store_columns<D>(at + step, keep ? (SPLIT ? acc : dv) : none, 1.f, hi);
+  };
+  if (a.parts > 1) write(a.dkv + (((long long)part * a.B * a.NKV + bk) * a.S + j) * 2 * D, D);
+  else write(a.dqkv + ((long long)b * a.S + j) * a.width + (a.NH + hk) * D, a.NKV * D);
 }
 
 // the parts' dK and dV, added in order: four columns a thread
@@ -754,24 +786,33 @@ __global__ __launch_bounds__(256) void k_rel_dkv(RelArgs a, long long n) {
 }
 
 // dtable[n][h]: the offsets' sums over batches and tiles, then over the offsets
-// of a bucket; one workgroup a head, every sum in a fixed order.
+// of a bucket; one workgroup a head, every sum in a fixed order. Latency bound:
+// a thread has up to twenty loads in flight.
 __global__ __launch_bounds__(1024) void k_rel_dtable(RelArgs a, int tiles) {
-  __shared__ float part[4][256];
+  __shared__ float part[16][320];
   __shared__ float sums[2 * GA_REL_MAX_DISTANCE + 1];
-  const int h = blockIdx.x, offs = 2 * a.far + 1, x = threadIdx.x & 255, y = threadIdx.x >> 8;
+  const int h = blockIdx.x, offs = 2 * a.far + 1, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int n = a.B * tiles;
-  for (int x0 = 0; x0 < offs; x0 += 256) {
-    float t = 0.f;
-    if (x0 + x < offs)
-      for (int w = y; w < n; w += 4)
-        t += a.doff[((long long)(w / tiles * a.NH + h) * tiles + w % tiles) * offs + x0 + x];
-    part[y][x] = t;
+  const float* p = a.doff + (long long)h * n * offs;
+  for (int x0 = 0; x0 < offs; x0 += 320) {
+    float t[5] = {};
+#pragma unroll 4
+    for (int w = wave; w < n; w += 16) {
+#pragma unroll
+      for (int i = 0; i < 5; ++i) t[i] += p[(long long)w * offs + min(x0 + 64 * i + lane, offs - 1)];
+    }
+#pragma unroll
+    for (int i = 0; i < 5; ++i) part[wave][64 * i + lane] = t[i];
     __syncthreads();
-    if (y == 0 && x0 + x < offs) sums[x0 + x] = (part[0][x] + part[1][x]) + (part[2][x] + part[3][x]);
+    if (threadIdx.x < 320 && x0 + threadIdx.x < offs) {
+      float s = 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s += part[i][threadIdx.x];
+      sums[x0 + threadIdx.x] = s;
+    }
     __syncthreads();
   }
-  const int lane = threadIdx.x & 63;
-  for (int bucket = threadIdx.x >> 6; bucket < a.buckets; bucket += 16) {
+  for (int bucket = wave; bucket < a.buckets; bucket += 16) {
     float t = 0.f;
     for (int e = lane; e < offs; e += 64)
       if (min(max(a.map[e], 0), a.buckets - 1) == bucket) t += sums[e];
@@ -999,11 +1040,12 @@ hipError_t backward(const RelArgs& a, hipStream_t s) {
   const size_t lds_q = 4 * KC * 2 * D + bias_bytes(a.far) + 16 + 32 * (2 * a.far + 1);
   const size_t lds_kv = 4 * KC * 2 * D + 16 * KC + bias_bytes(a.far);
   hipError_t e = allow(k_rel_bwd_q<D>, lds_q);
-  if (e == hipSuccess) e = allow(k_rel_bwd_kv<D>, lds_kv);
+  constexpr bool SPLIT = D == 128;
+  if (e == hipSuccess) e = allow(k_rel_bwd_kv<D, SPLIT>, lds_kv);
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL((k_rel_bwd_q<D>), dim3(a.B * a.NH * tiles), dim3(256), lds_q, s, a, tiles);
   if ((e = hipGetLastError()) != hipSuccess) return e;
-  hipLaunchKernelGGL((k_rel_bwd_kv<D>), dim3(a.B * a.NKV * a.parts * tiles), dim3(256), lds_kv, s, a, tiles);
+  hipLaunchKernelGGL((k_rel_bwd_kv<D, SPLIT>), dim3(a.B * a.NKV * a.parts * tiles), dim3(SPLIT ? 512 : 256), lds_kv, s, a, tiles);
   if ((e = hipGetLastError()) != hipSuccess) return e;
   if (a.parts > 1) {
     const long long n = (long long)a.B * a.NKV * a.S * (D / 2);

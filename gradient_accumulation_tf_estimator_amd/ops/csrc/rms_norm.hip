@@ -35,19 +35,6 @@ struct Fp16 { typedef _Float16 t; };
 struct Fp32 { typedef float t; };
 
 template <typename E>
-__device__ __forceinline__ void load8(const E* p, float* f) {
-  typedef __attribute__((ext_vector_type(8))) E e8;
-  const e8 v = *(const e8*)p;
-#pragma unroll
-  for (int k = 0; k < 8; ++k) f[k] = (float)v[k];
-}
-template <>
-__device__ __forceinline__ void load8<float>(const float* p, float* f) {
-  const f4 a = *(const f4*)p, b = *(const f4*)(p + 4);
-#pragma unroll
-  for (int k = 0; k < 4; ++k) { f[k] = a[k]; f[4 + k] = b[k]; }
-}
-template <typename E>
 __device__ __forceinline__ void store8(E* p, const float* f) {
   typedef __attribute__((ext_vector_type(8))) E e8;
   e8 v;
@@ -74,25 +61,30 @@ __device__ __forceinline__ int column(int v, int e, int t) {
   return MODE == SCALAR ? (v * 8 + e) * NT + t : (v * NT + t) * 8 + e;
 }
 
+// A thread's part of a row as it lies in memory; converted where it is used, so
+// that the next row can wait in few registers.
 template <typename E, int NT, int NV, int MODE>
-__device__ __forceinline__ void load_row(const E* row, int H, int t, float (*f)[8]) {
+struct Row {
+  typedef __attribute__((ext_vector_type(8))) E e8;
+  e8 x[NV];
+  __device__ __forceinline__ void load(const void* base, long long at, int H, int t) {
+    const E* row = (const E*)base + at;
 #pragma unroll
-  for (int v = 0; v < NV; ++v) {
-    if (MODE == VEC) {
-      const int c = column<NT, MODE>(v, 0, t);
-      if (c < H) load8<E>(row + c, f[v]);
-      else
+    for (int v = 0; v < NV; ++v) {
+      if (MODE == VEC) {
+        const int c = column<NT, MODE>(v, 0, t);
+        x[v] = c < H ? *(const e8*)(row + c) : (e8){};
+      } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[v][e] = 0.f;
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int c = column<NT, MODE>(v, e, t);
-        f[v][e] = c < H ? (float)row[c] : 0.f;
+        for (int e = 0; e < 8; ++e) {
+          const int c = column<NT, MODE>(v, e, t);
+          x[v][e] = c < H ? row[c] : (E)0.f;
+        }
       }
     }
   }
-}
+  __device__ __forceinline__ float at(int v, int e) const { return (float)x[v][e]; }
+};
 template <typename E, int NT, int NV, int MODE>
 __device__ __forceinline__ void store_row(E* row, int H, int t, const float (*f)[8]) {
 #pragma unroll
@@ -132,42 +124,44 @@ __device__ __forceinline__ float over_row(float s, float* lds) {
   return s;
 }
 
-// A block holds 256 / NT rows; grid-stride over the rows. The reduction's
-// floats alternate between two halves, so one barrier a row is enough.
+// A block holds 256 / NT rows; grid-stride over the rows, the next one's loads
+// issued before this one's reduction. The reduction's floats alternate between
+// two halves, so one barrier a row is enough.
 template <typename E, int NT, int NV, int MODE>
 __global__ __launch_bounds__(256) void k_rms_fwd(RmsArgs a) {
   constexpr int RB = 256 / NT;
   __shared__ float lds[2][4];
   const int t = threadIdx.x % NT;
+  const long long first = (long long)blockIdx.x * RB + threadIdx.x / NT, step = (long long)gridDim.x * RB;
+  typedef Row<E, NT, NV, MODE> R;
+  R w, x, r;
+  w.load(a.w, 0, a.H, t);
+  auto fetch = [&](long long row) {
+    x.load(a.x, row * a.x_stride, a.H, t);
+    if (a.res) r.load(a.res, row * a.res_stride, a.H, t);
+  };
+  if (first < a.R) fetch(first);
   int turn = 0;
-  for (long long row = (long long)blockIdx.x * RB + threadIdx.x / NT; row < a.R;
-       row += (long long)gridDim.x * RB, turn ^= 1) {
-    float h[NV][8];
-    load_row<E, NT, NV, MODE>((const E*)a.x + row * a.x_stride, a.H, t, h);
-    if (a.res) {
-      float r[NV][8];
-      load_row<E, NT, NV, MODE>((const E*)a.res + row * a.res_stride, a.H, t, r);
+  for (long long row = first; row < a.R; row += step, turn ^= 1) {
+    float h[NV][8], s = 0.f;
 #pragma unroll
-      for (int v = 0; v < NV; ++v)
+    for (int v = 0; v < NV; ++v)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) h[v][e] += r[v][e];
-      store_row<E, NT, NV, MODE>((E*)a.h + row * a.H, a.H, t, h);
-    }
-    float s = 0.f;
+      for (int e = 0; e < 8; ++e) h[v][e] = a.res ? x.at(v, e) + r.at(v, e) : x.at(v, e);
+    if (row + step < a.R) fetch(row + step);
+    if (a.res) store_row<E, NT, NV, MODE>((E*)a.h + row * a.H, a.H, t, h);
 #pragma unroll
     for (int v = 0; v < NV; ++v)
 #pragma unroll
       for (int e = 0; e < 8; ++e) s = fmaf(h[v][e], h[v][e], s);
     s = over_row<NT, Sum>(s, lds[turn]);
     const float rstd = 1.f / sqrtf(s / (float)a.H + a.eps);
-    float w[NV][8];
-    load_row<E, NT, NV, MODE>((const E*)a.w, a.H, t, w);
 #pragma unroll
     for (int v = 0; v < NV; ++v)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) h[v][e] = h[v][e] * rstd * w[v][e];
+      for (int e = 0; e < 8; ++e) h[v][e] = h[v][e] * rstd * w.at(v, e);
     store_row<E, NT, NV, MODE>((E*)a.y + row * a.H, a.H, t, h);
-    if (t == 0 && a.rstd) a.rstd[row] = rstd;
+    if (t == 0) a.rstd[row] = rstd;
   }
 }
 
@@ -176,46 +170,65 @@ __global__ __launch_bounds__(256) void k_rms_bwd(RmsArgs a) {
   constexpr int RB = 256 / NT;
   __shared__ float lds[2][4];
   const int t = threadIdx.x % NT;
-  float w[NV][8], dw[NV][8];
-  load_row<E, NT, NV, MODE>((const E*)a.w, a.H, t, w);
+  const long long first = (long long)blockIdx.x * RB + threadIdx.x / NT, step = (long long)gridDim.x * RB;
+  typedef Row<E, NT, NV, MODE> R;
+  R w, x, dy, dh;
+  float dw[NV][8], rs = 0.f;
+  w.load(a.w, 0, a.H, t);
 #pragma unroll
   for (int v = 0; v < NV; ++v)
 #pragma unroll
     for (int e = 0; e < 8; ++e) dw[v][e] = 0.f;
+  auto fetch = [&](long long row) {
+    x.load(a.x, row * a.x_stride, a.H, t);
+    dy.load(a.dy, row * a.dy_stride, a.H, t);
+    rs = a.rstd[row];
+  };
+  if (first < a.R) fetch(first);
   int turn = 0;
-  for (long long row = (long long)blockIdx.x * RB + threadIdx.x / NT; row < a.R;
-       row += (long long)gridDim.x * RB, turn ^= 1) {
-    float n[NV][8], g[NV][8];
-    load_row<E, NT, NV, MODE>((const E*)a.x + row * a.x_stride, a.H, t, n);
-    load_row<E, NT, NV, MODE>((const E*)a.dy + row * a.dy_stride, a.H, t, g);
-    const float rstd = a.rstd[row];
-    float s = 0.f;
+  for (long long row = first; row < a.R; row += step, turn ^= 1) {
+    float n[NV][8], g[NV][8], s = 0.f;
+    const float rstd = rs;
+    if (a.dh) dh.load(a.dh, row * a.dh_stride, a.H, t);
 #pragma unroll
     for (int v = 0; v < NV; ++v)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        n[v][e] *= rstd;
-        dw[v][e] = fmaf(g[v][e], n[v][e], dw[v][e]);
-        g[v][e] *= w[v][e];
+        n[v][e] = x.at(v, e) * rstd;
+        dw[v][e] = fmaf(dy.at(v, e), n[v][e], dw[v][e]);
+        g[v][e] = dy.at(v, e) * w.at(v, e);
         s = fmaf(g[v][e], n[v][e], s);
       }
+    if (row + step < a.R) fetch(row + step);
     s = over_row<NT, Sum>(s, lds[turn]) / (float)a.H;
 #pragma unroll
     for (int v = 0; v < NV; ++v)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) g[v][e] = rstd * fmaf(-n[v][e], s, g[v][e]);
-    if (a.dh) {
-      load_row<E, NT, NV, MODE>((const E*)a.dh + row * a.dh_stride, a.H, t, n);
+      for (int e = 0; e < 8; ++e) {
+        g[v][e] = rstd * fmaf(-n[v][e], s, g[v][e]);
+        if (a.dh) g[v][e] += dh.at(v, e);
+      }
+    store_row<E, NT, NV, MODE>((E*)a.y + row * a.H, a.H, t, g);
+  }
+  // one slab a block: [gridDim.x][H]; the block's waves add theirs up in order
+  if (RB > 1) {
+    __shared__ float join[RB > 1 ? RB - 1 : 1][NT * NV * 8];
+    const int w = threadIdx.x / NT;
+    if (w > 0)
 #pragma unroll
       for (int v = 0; v < NV; ++v)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) g[v][e] += n[v][e];
-    }
-    store_row<E, NT, NV, MODE>((E*)a.y + row * a.H, a.H, t, g);
+        for (int e = 0; e < 8; ++e) join[w - 1][(v * 8 + e) * NT + t] = dw[v][e];
+    __syncthreads();
+    if (w > 0) return;
+#pragma unroll
+    for (int i = 0; i < RB - 1; ++i)
+#pragma unroll
+      for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dw[v][e] += join[i][(v * 8 + e) * NT + t];
   }
-  // one slab a row group: [gridDim.x * RB][H]
-  float* slab = a.slabs + ((long long)blockIdx.x * RB + threadIdx.x / NT) * a.H;
-  store_row<float, NT, NV, MODE>(slab, a.H, t, dw);
+  store_row<float, NT, NV, MODE>(a.slabs + (long long)blockIdx.x * a.H, a.H, t, dw);
 }
 
 // dw[c] = sum over slabs; 16 columns x 16 slab groups a block, joined in LDS in
@@ -225,8 +238,10 @@ __global__ __launch_bounds__(256) void k_rms_dw(const float* slabs, int n, int H
   __shared__ float lds[16][17];
   const int c = blockIdx.x * 16 + (threadIdx.x & 15), g = threadIdx.x >> 4;
   float s = 0.f;
-  if (c < H)
+  if (c < H) {
+#pragma unroll 16
     for (int i = g; i < n; i += 16) s += slabs[(long long)i * H + c];
+  }
   lds[g][threadIdx.x & 15] = s;
   __syncthreads();
   if (g == 0 && c < H) {
@@ -247,35 +262,36 @@ __global__ __launch_bounds__(256) void k_rms_fp8(RmsArgs a) {
   constexpr int RB = 256 / NT;
   __shared__ float lds[4][4];
   const int t = threadIdx.x % NT;
+  const long long first = (long long)blockIdx.x * RB + threadIdx.x / NT, step = (long long)gridDim.x * RB;
+  typedef Row<E, NT, NV, MODE> R;
+  R w, x, r;
+  w.load(a.w, 0, a.H, t);
+  auto fetch = [&](long long row) {
+    x.load(a.x, row * a.x_stride, a.H, t);
+    if (a.res) r.load(a.res, row * a.res_stride, a.H, t);
+  };
+  if (first < a.R) fetch(first);
   int turn = 0;
-  for (long long row = (long long)blockIdx.x * RB + threadIdx.x / NT; row < a.R;
-       row += (long long)gridDim.x * RB, turn ^= 2) {
-    float h[NV][8];
-    load_row<E, NT, NV, MODE>((const E*)a.x + row * a.x_stride, a.H, t, h);
-    if (a.res) {
-      float r[NV][8];
-      load_row<E, NT, NV, MODE>((const E*)a.res + row * a.res_stride, a.H, t, r);
+  for (long long row = first; row < a.R; row += step, turn ^= 2) {
+    float h[NV][8], s = 0.f, m[NV], all = 0.f;
 #pragma unroll
-      for (int v = 0; v < NV; ++v)
+    for (int v = 0; v < NV; ++v)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) h[v][e] += r[v][e];
-      store_row<E, NT, NV, MODE>((E*)a.h + row * a.H, a.H, t, h);
-    }
-    float s = 0.f;
+      for (int e = 0; e < 8; ++e) h[v][e] = a.res ? x.at(v, e) + r.at(v, e) : x.at(v, e);
+    if (row + step < a.R) fetch(row + step);
+    if (a.res) store_row<E, NT, NV, MODE>((E*)a.h + row * a.H, a.H, t, h);
 #pragma unroll
     for (int v = 0; v < NV; ++v)
 #pragma unroll
       for (int e = 0; e < 8; ++e) s = fmaf(h[v][e], h[v][e], s);
     s = over_row<NT, Sum>(s, lds[turn]);
     const float rstd = 1.f / sqrtf(s / (float)a.H + a.eps);
-    float w[NV][8], m[NV], all = 0.f;
-    load_row<E, NT, NV, MODE>((const E*)a.w, a.H, t, w);
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       m[v] = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        h[v][e] = h[v][e] * rstd * w[v][e];
+        h[v][e] = h[v][e] * rstd * w.at(v, e);
         m[v] = Max::of(m[v], fabsf(h[v][e]));
       }
       all = Max::of(all, m[v]);
@@ -357,10 +373,10 @@ inline int rows_a_block(int H) { return H <= 1024 ? 4 : 1; }
 
 int rms_blocks(long long R, int H, bool backward) {
   const long long need = (R + rows_a_block(H) - 1) / rows_a_block(H);
-  const long long most = backward ? 512 : 4096;
+  const long long most = backward ? 1024 : 4096;
   return (int)(need < most ? need : most);
 }
-int rms_slabs(long long R, int H) { return rms_blocks(R, H, true) * rows_a_block(H); }
+int rms_slabs(long long R, int H) { return rms_blocks(R, H, true); }
 
 hipError_t rms_forward(int type, bool vec, const RmsArgs& a, hipStream_t s) {
   return by_type(FWD, type, vec ? VEC : SCALAR, a, rms_blocks(a.R, a.H, false), s);

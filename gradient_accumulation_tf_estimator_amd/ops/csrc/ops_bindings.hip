@@ -125,8 +125,53 @@ std::vector<at::Tensor> rms_norm_bwd(at::Tensor dy, MaybeTensor dh, at::Tensor h
   return {dx, dw};
 }
 
+// [rows, hidden] with neighbouring columns; a copy only where needed
+at::Tensor as_rows(const at::Tensor& t) {
+  auto r = t.dim() == 2 ? t : t.reshape({-1, t.size(-1)});
+  return r.size(1) == 1 || r.stride(1) == 1 ? r : r.contiguous();
+}
+MaybeTensor as_rows(const MaybeTensor& t) { return t ? MaybeTensor(as_rows(*t)) : t; }
+MaybeTensor maybe(const at::Tensor& t) { return t.defined() ? MaybeTensor(t) : MaybeTensor(); }
+
+// The autograd node lives here: in Python its forward and backward cost more
+// than the kernels on a small batch. `dw_acc`: an fp32 slice that the weight's
+// gradient is added to instead of being returned.
+struct AddRmsNorm : public torch::autograd::Function<AddRmsNorm> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, at::Tensor x, MaybeTensor res,
+                                                at::Tensor w, double eps, MaybeTensor dw_acc) {
+    w = w.contiguous();
+    auto r = rms_norm_fwd(as_rows(x), as_rows(res), w, eps);
+    ctx->save_for_backward({r[1], w, r[2]});
+    ctx->set_materialize_grads(false);
+    ctx->saved_data["res"] = res.has_value();
+    if (dw_acc) ctx->saved_data["acc"] = *dw_acc;
+    return {r[0].view(x.sizes()), res ? r[1].view(x.sizes()) : x};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const auto dy = grads[0], dh = grads[1];
+    at::Tensor dx = dh, dw;
+    if (dy.defined()) {  // y was used
+      const auto acc = ctx->saved_data.find("acc");
+      auto r = rms_norm_bwd(as_rows(dy), as_rows(maybe(dh)), saved[0], saved[1], saved[2],
+                            acc == ctx->saved_data.end() ? MaybeTensor() : MaybeTensor(acc->second.toTensor()));
+      dx = r[0].view(dy.sizes());
+      dw = r[1];
+    }
+    return {dx, ctx->saved_data["res"].toBool() ? dx : at::Tensor(), dw, at::Tensor(), at::Tensor()};
+  }
+};
+
+std::vector<at::Tensor> add_rms_norm(at::Tensor x, MaybeTensor res, at::Tensor w, double eps, MaybeTensor dw_acc) {
+  return AddRmsNorm::apply(x, res, w, eps, dw_acc);
+}
+
 std::vector<at::Tensor> rms_norm_fp8(at::Tensor x, MaybeTensor res, at::Tensor w, double eps, int64_t group) {
   bool vec;
+  x = as_rows(x);
+  res = as_rows(res);
+  w = w.contiguous();
   RmsArgs a = norm_args(x, w, eps, vec);
   const c10::OptionalDeviceGuard guard(x.device());
   TORCH_CHECK(group == 0 || group == 32 || group == 64 || group == 128, "group must be 0 (a row), 32, 64 or 128");
@@ -337,6 +382,42 @@ std::vector<at::Tensor> rel_attn_bwd(at::Tensor dout, at::Tensor qkv, at::Tensor
   return {dqkv, dtable};
 }
 
+at::Tensor aligned(const at::Tensor& t) {
+  const auto c = t.contiguous();
+  return aligned16(c.data_ptr()) ? c : c.clone();
+}
+
+struct RelAttention : public torch::autograd::Function<RelAttention> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, at::Tensor qkv, at::Tensor table, at::Tensor map,
+                            MaybeTensor mask, int64_t NH, int64_t NKV, bool causal, double scale) {
+    qkv = aligned(qkv);
+    table = table.contiguous();
+    auto r = rel_attn_fwd(qkv, NH, NKV, table, map, mask, causal, scale, true);
+    ctx->save_for_backward({qkv, table, map, mask ? *mask : at::Tensor(), r[0], r[1]});
+    ctx->saved_data["NH"] = NH;
+    ctx->saved_data["NKV"] = NKV;
+    ctx->saved_data["causal"] = causal;
+    ctx->saved_data["scale"] = scale;
+    return r[0];
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    const auto s = ctx->get_saved_variables();
+    auto r = rel_attn_bwd(aligned(grads[0]), s[0], s[4], s[5], ctx->saved_data["NH"].toInt(), ctx->saved_data["NKV"].toInt(),
+                          s[1], s[2], maybe(s[3]), ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble());
+    at::Tensor none;
+    return {r[0], r[1], none, none, none, none, none, none};
+  }
+};
+
+// with gradients recorded, the forward keeps what the backward needs
+at::Tensor rel_attention(at::Tensor qkv, at::Tensor table, at::Tensor map, MaybeTensor mask, int64_t NH, int64_t NKV,
+                         bool causal, double scale) {
+  if (at::GradMode::is_enabled() && (qkv.requires_grad() || table.requires_grad()))
+    return RelAttention::apply(qkv, table, map, mask, NH, NKV, causal, scale);
+  return rel_attn_fwd(aligned(qkv), NH, NKV, table.contiguous(), map, mask, causal, scale, false)[0];
+}
+
 // q [B, Sq, NH, D], caches [B, S, NKV, D] of any strides with contiguous, 16-byte aligned rows
 at::Tensor rel_attn_token(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor table, at::Tensor map,
                           at::Tensor lengths, double scale) {
@@ -389,11 +470,9 @@ at::Tensor rel_attn_token(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor t
 }  // namespace
 
 void register_ops(pybind11::module_& mod) {
-  mod.def("rms_norm_fwd", &rms_norm_fwd, "x (+ residual) -> y, h, rstd");
-  mod.def("rms_norm_bwd", &rms_norm_bwd, "dy (+ dh) -> dx, dw (or dw added to an fp32 slice)");
+  mod.def("add_rms_norm", &add_rms_norm, "x (+ residual) -> y, h, with gradients");
   mod.def("rms_norm_fp8", &rms_norm_fp8, "x (+ residual) -> e4m3 values, scales, h");
-  mod.def("rel_attn_fwd", &rel_attn_fwd, "packed qkv + bucket bias -> out, lse");
-  mod.def("rel_attn_bwd", &rel_attn_bwd, "-> packed dqkv, dtable");
+  mod.def("rel_attention", &rel_attention, "attention over packed qkv with a bucket bias, with gradients");
   mod.def("rel_attn_token", &rel_attn_token, "new tokens over a K/V cache with a bucket bias");
   mod.def("global_norm", &global_norm, "norm over many tensors; with outputs, clipped copies");
 }

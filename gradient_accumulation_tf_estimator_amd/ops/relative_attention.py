@@ -29,7 +29,6 @@ from typing import Optional
 
 import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
 
 from . import require_hip
 
@@ -93,32 +92,6 @@ def _check_gpu(t, head_dim):
         raise ValueError(f"the attention kernels take head size 64 or 128, got {head_dim}")
 
 
-def _aligned(t):
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
-
-
-class _RelativeAttentionFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, qkv, table, buckets, mask8, nh, nkv, causal, scale):
-        hip = require_hip()
-        qkv, table = _aligned(qkv), table.contiguous()
-        out, lse = hip.rel_attn_fwd(qkv, nh, nkv, table, buckets, mask8, causal, scale, True)
-        ctx.save_for_backward(qkv, table, buckets, mask8, out, lse)
-        ctx.how = nh, nkv, causal, scale
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dout):
-        hip = require_hip()
-        qkv, table, buckets, mask8, out, lse = ctx.saved_tensors
-        nh, nkv, causal, scale = ctx.how
-        dqkv, dtable = hip.rel_attn_bwd(_aligned(dout), qkv, out, lse, nh, nkv, table, buckets,
-                                        mask8, causal, scale)
-        return dqkv, dtable, None, None, None, None, None, None
-
-
 def _bias(table, buckets, rows, cols):
     """[NH, rows, cols] for positions of queries and keys."""
     far = buckets.numel() // 2
@@ -175,10 +148,7 @@ def fused_relative_attention(qkv: torch.Tensor, nh: int, table: torch.Tensor, bu
     _check_gpu(qkv, D)
     if mask8 is not None:
         mask8 = (mask8.view(torch.uint8) if mask8.dtype == torch.bool else mask8).contiguous()
-    if torch.is_grad_enabled() and (qkv.requires_grad or table.requires_grad):
-        return _RelativeAttentionFn.apply(qkv, table, buckets.contiguous(), mask8, nh, nkv, bool(causal), scale)
-    return require_hip().rel_attn_fwd(_aligned(qkv.detach()), nh, nkv, table.detach().contiguous(), buckets.contiguous(),
-                                      mask8, bool(causal), scale, False)[0]
+    return require_hip().rel_attention(qkv, table, buckets.contiguous(), mask8, nh, nkv, causal, scale)
 
 
 def relative_attention_decode(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor,

@@ -20,18 +20,11 @@ from typing import Optional, Tuple
 
 import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
 
 from . import require_hip
 
 FP8_MAX = 448.0  # the largest finite e4m3 value
 GROUPS = (0, 32, 64, 128)
-
-
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """[rows, hidden] with neighbouring columns; a copy only where needed."""
-    t = t.reshape(-1, t.shape[-1])
-    return t if t.shape[1] == 1 or t.stride(1) == 1 else t.contiguous()
 
 
 def _check(x, weight, residual):
@@ -47,33 +40,6 @@ def _check(x, weight, residual):
                              f"({x.dtype}, {x.device}), got ({t.dtype}, {t.device})")
 
 
-class _AddRMSNormFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, residual, weight, eps, module):
-        hip = require_hip()
-        y, h, rstd = hip.rms_norm_fwd(_rows(x), None if residual is None else _rows(residual),
-                                      weight.contiguous(), eps)
-        ctx.save_for_backward(h, weight, rstd)
-        ctx.set_materialize_grads(False)
-        ctx.module = module
-        ctx.has_res = residual is not None
-        return y.view(x.shape), (h.view(x.shape) if ctx.has_res else x)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy, dh):
-        hip = require_hip()
-        h, weight, rstd = ctx.saved_tensors
-        acc = getattr(ctx.module, "_accum_view", None)
-        if dy is None:  # y was not used
-            dx, dw = dh, None
-        else:
-            dx, dw = hip.rms_norm_bwd(_rows(dy), None if dh is None else _rows(dh), h,
-                                      weight.contiguous(), rstd, acc)
-            dx = dx.view(dy.shape)
-        return dx, dx if ctx.has_res else None, dw, None, None
-
-
 def _plain(x, weight, residual, eps):
     up = torch.promote_types(x.dtype, torch.float32)
     h = x if residual is None else x + residual
@@ -83,14 +49,14 @@ def _plain(x, weight, residual, eps):
 
 
 def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None, *,
-                 eps: float = 1e-6, _module=None) -> Tuple[torch.Tensor, torch.Tensor]:
+                 eps: float = 1e-6, _dw_acc: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """x, residual [..., hidden]; weight [hidden], all of one dtype -> (y, h).
     Without a residual, h is x."""
     _check(x, weight, residual)
     if eps < 0:
         raise ValueError(f"eps must not be negative, got {eps}")
     if x.is_cuda:
-        return _AddRMSNormFn.apply(x, residual, weight, float(eps), _module)
+        return tuple(require_hip().add_rms_norm(x, residual, weight, eps, _dw_acc))
     y, h = _plain(x, weight, residual, eps)
     return y.to(x.dtype), h
 
@@ -112,8 +78,7 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch
         raise RuntimeError("rms_norm_fp8 has no gradient: call it under torch.no_grad()")
     groups = x.shape[-1] // group if group else 1
     if x.is_cuda:
-        q, s, h = require_hip().rms_norm_fp8(_rows(x), None if residual is None else _rows(residual),
-                                             weight.contiguous(), float(eps), group)
+        q, s, h = require_hip().rms_norm_fp8(x, residual, weight, eps, group)
     else:
         y, h = _plain(x, weight, residual, eps)
         y = y.reshape(x[..., 0].numel(), groups, x.shape[-1] // groups)
@@ -139,7 +104,7 @@ class FusedAddRMSNorm(nn.Module):
     def forward(self, x, residual=None, return_sum: bool = False):
         if self._accum_view is not None and not x.is_cuda:
             raise RuntimeError("bound FusedAddRMSNorm got a non-GPU input")
-        y, h = add_rms_norm(x, self.weight, residual, eps=self.eps, _module=self)
+        y, h = add_rms_norm(x, self.weight, residual, eps=self.eps, _dw_acc=self._accum_view)
         return (y, h) if return_sum else y
 
     def forward_fp8(self, x, residual=None, group: int = 0):

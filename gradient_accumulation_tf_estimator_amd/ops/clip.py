@@ -28,13 +28,16 @@ Tensors = Sequence[Optional[torch.Tensor]]
 def _present(tensors: Tensors) -> List[torch.Tensor]:
     if isinstance(tensors, torch.Tensor):
         raise TypeError("expected a list of tensors")
-    got = [t.detach() for t in tensors if t is not None]
-    for t in got:
+    return [t for t in tensors if t is not None]
+
+
+def _plain_norm(tensors: List[torch.Tensor]) -> torch.Tensor:
+    for t in tensors:
         if t.dtype not in (torch.float32, torch.bfloat16, torch.float16):
             raise ValueError(f"tensors must be fp32, bf16 or fp16, got {t.dtype}")
-        if t.device != got[0].device:
+        if t.device != tensors[0].device:
             raise ValueError("tensors must be on one device")
-    return got
+    return torch.stack([t.detach().double().square().sum() for t in tensors]).sum().sqrt()
 
 
 def global_norm(tensors: Tensors) -> torch.Tensor:
@@ -43,8 +46,8 @@ def global_norm(tensors: Tensors) -> torch.Tensor:
     if not got:
         return torch.zeros(())
     if got[0].is_cuda:
-        return require_hip().global_norm(got, [], 1.0)
-    return torch.stack([t.double().square().sum() for t in got]).sum().sqrt().float()
+        return require_hip().global_norm(got, [], False, 1.0)[0]
+    return _plain_norm(got).float()
 
 
 def clip_by_global_norm(tensors: Tensors, clip_norm: float, *,
@@ -56,23 +59,32 @@ def clip_by_global_norm(tensors: Tensors, clip_norm: float, *,
     if not (clip_norm > 0):
         raise ValueError(f"clip_norm must be positive, got {clip_norm}")
     got = _present(tensors)
-    if out is None:
-        new = [None if t is None else torch.empty_like(t, requires_grad=False) for t in tensors]
-    else:
-        new = list(out)
-        if len(new) != len(tensors) or any((a is None) != (b is None) for a, b in zip(new, tensors)):
-            raise ValueError("out must have an entry for each tensor, and None where it has None")
+    if out is not None and (len(out) != len(tensors) or any((a is None) != (b is None) for a, b in zip(out, tensors))):
+        raise ValueError("out must have an entry for each tensor, and None where it has None")
     if not got:
-        return new, torch.zeros(())
-    dst = [t.detach() for t in new if t is not None]
+        return [None] * len(tensors), torch.zeros(())
+    dst = [] if out is None else _present(out)
     if got[0].is_cuda:
-        return new, require_hip().global_norm(got, dst, float(clip_norm))
-    norm = torch.stack([t.double().square().sum() for t in got]).sum().sqrt()
+        norm, dst = require_hip().global_norm(got, dst, True, float(clip_norm))
+    else:
+        norm, dst = _plain_clip(got, dst, clip_norm)
+    if out is not None:
+        return list(out), norm
+    if len(dst) < len(tensors):
+        rest = iter(dst)
+        dst = [None if t is None else next(rest) for t in tensors]
+    return dst, norm
+
+
+@torch.no_grad()
+def _plain_clip(got, dst, clip_norm):
+    norm = _plain_norm(got)
     n = float(norm)
     coef = math.nan if not math.isfinite(n) else 1.0 if n <= clip_norm else clip_norm / n
     coef = torch.tensor(coef, dtype=torch.float32)
+    dst = dst or [torch.empty_like(t) for t in got]
     for d, t in zip(dst, got):
         if d.shape != t.shape or d.dtype != t.dtype or d.device != t.device:
             raise ValueError("an output must have its tensor's device, dtype and shape")
         d.copy_(t.float() * coef)
-    return new, norm.float()
+    return norm.float(), dst

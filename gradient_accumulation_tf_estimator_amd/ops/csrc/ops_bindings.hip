@@ -217,30 +217,38 @@ void check_apart(const std::vector<at::Tensor>& ins, const std::vector<at::Tenso
   }
 }
 
-// Norm of all tensors; with `outs`, outs[i] = ins[i] * min(1, clip / norm).
-// Tensors are taken as their memory, whatever the order of their dimensions;
-// an output has to have its input's strides.
-at::Tensor global_norm(std::vector<at::Tensor> ins, std::vector<at::Tensor> outs, double clip) {
-  TORCH_CHECK(!ins.empty(), "global_norm needs at least one tensor");
-  const bool write = !outs.empty();
-  TORCH_CHECK(!write || outs.size() == ins.size(), "one output for each tensor");
-  TORCH_CHECK(!write || clip > 0, "clip_norm must be positive");
+// -> norm of all tensors, and with `write` outs[i] = ins[i] * min(1, clip / norm)
+// (new tensors where outs is empty). Tensors are taken as their memory,
+// whatever the order of their dimensions; an output has to have its input's
+// strides.
+std::tuple<at::Tensor, std::vector<at::Tensor>> global_norm(std::vector<at::Tensor> ins, std::vector<at::Tensor> outs,
+                                                            bool write, double clip) {
+  TORCH_CHECK_VALUE(!ins.empty(), "global_norm needs at least one tensor");
+  TORCH_CHECK_VALUE(!write || clip > 0, "clip_norm must be positive");
   const auto dev = ins[0].device();
-  TORCH_CHECK(ins[0].is_cuda(), "tensors must be on a GPU");
+  TORCH_CHECK_VALUE(ins[0].is_cuda(), "tensors must be on a GPU");
   const c10::OptionalDeviceGuard guard(dev);
   long long total = 0;
   for (size_t i = 0; i < ins.size(); ++i) {
-    TORCH_CHECK(ins[i].device() == dev, "tensors must be on one device");
-    type_of(ins[i], "tensor");
+    TORCH_CHECK_VALUE(ins[i].device() == dev, "tensors must be on one device");
+    const auto t = ins[i].scalar_type();
+    TORCH_CHECK_VALUE(t == at::kFloat || t == at::kBFloat16 || t == at::kHalf, "tensors must be fp32, bf16 or fp16, got ", t);
     TORCH_CHECK(ins[i].is_non_overlapping_and_dense(), "tensor ", i,
                 " has gaps or overlaps in memory: pass a contiguous copy");
-    if (write)
+    total += ins[i].numel();
+  }
+  if (write && outs.empty()) {
+    for (const auto& t : ins) outs.push_back(at::empty_like(t));
+  } else if (write) {
+    TORCH_CHECK_VALUE(outs.size() == ins.size(), "one output for each tensor");
+    for (size_t i = 0; i < ins.size(); ++i)
       TORCH_CHECK(outs[i].device() == dev && outs[i].scalar_type() == ins[i].scalar_type() &&
                   outs[i].sizes() == ins[i].sizes() && outs[i].strides() == ins[i].strides(),
                   "output ", i, " must have its tensor's device, dtype, shape and strides");
-    total += ins[i].numel();
+    check_apart(ins, outs);
+    for (auto& t : outs)
+      if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();  // written behind autograd's back
   }
-  if (write) check_apart(ins, outs);
   // about 4096 blocks for large sets, at least 8192 elements a block
   long long chunk = (total / 4096 + 2047) / 2048 * 2048;
   if (chunk < 8192) chunk = 8192;
@@ -279,7 +287,7 @@ at::Tensor global_norm(std::vector<at::Tensor> ins, std::vector<at::Tensor> outs
                "global_norm");
   if (write)
     for (const auto& a : launches) check_launch(clip_scale(a, r + 1, s), "clip_by_global_norm");
-  return result.select(0, 0);
+  return {result.select(0, 0), outs};
 }
 
 // ---------------- attention with a relative position bias ----------------

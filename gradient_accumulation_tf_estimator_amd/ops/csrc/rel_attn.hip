@@ -845,18 +845,6 @@ __global__ __launch_bounds__(256) void k_rel_token(RelTokenArgs a, int row_tiles
   const int pos = row < rows ? len - a.Sq + tok : -1;  // the last key of this row
   const int pos0 = len - a.Sq + rt * 32 / group;       // the first row's
 
-  for (int x = threadIdx.x; x <= a.far; x += 256) map[x] = min(max(a.map[x], 0), a.buckets - 1);
-  for (int x = threadIdx.x; x < a.buckets * group; x += 256)
-    table[x] = as_bias(a.table[(long long)(x / group) * a.NH + hk * group + x % group], a.scale);
-
-  b8 q[D / 16];
-  const __bf16* qp = a.q + b * a.q_b + tok * a.q_s + h * a.q_h;
-#pragma unroll
-  for (int t = 0; t < D / 16; ++t) q[t] = *(const b8*)(qp + 16 * t + 8 * hi);
-  __syncthreads();
-  const int mine = h - hk * group;
-  const float low = table[map[0] * group + mine];
-
   // keys in units of 32, spread evenly over the waves of all splits
   const int units = (len + 31) / 32, waves = a.splits * 4, w = split * 4 + wave;
   const int u0 = (int)((long long)units * w / waves), u1 = (int)((long long)units * (w + 1) / waves);
@@ -875,10 +863,22 @@ __global__ __launch_bounds__(256) void k_rel_token(RelTokenArgs a, int row_tiles
       vf[n] = *(const b8*)(v + min(r, len - 1) * a.v_s + x % (D / 8) * 8);
     }
   };
+  // the first keys are on their way while the bias is staged
+  if (u0 < u1) fetch(u0);
+  b8 q[D / 16];
+  const __bf16* qp = a.q + b * a.q_b + tok * a.q_s + h * a.q_h;
+#pragma unroll
+  for (int t = 0; t < D / 16; ++t) q[t] = *(const b8*)(qp + 16 * t + 8 * hi);
+  for (int x = threadIdx.x; x <= a.far; x += 256) map[x] = min(max(a.map[x], 0), a.buckets - 1);
+  for (int x = threadIdx.x; x < a.buckets * group; x += 256)
+    table[x] = as_bias(a.table[(long long)(x / group) * a.NH + hk * group + x % group], a.scale);
+  __syncthreads();
+  const int mine = h - hk * group;
+  const float low = table[map[0] * group + mine];
+
   f16 o[D / 32] = {};
   float m = -INF, l = 0.f;
   const float c2 = a.scale * LOG2E;
-  if (u0 < u1) fetch(u0);
   for (int u = u0; u < u1; ++u) {
     const int j0 = u * 32;
     const b8 zero = {};
@@ -1002,14 +1002,30 @@ __global__ __launch_bounds__(D) void k_rel_join(RelTokenArgs a, int row_tiles) {
   const long long rest = ((long long)b * a.NKV + hk) * row_tiles + at / 32;
   const float* p = a.parts + (rest * a.splits * 32 + at % 32) * (D + 2);
   const long long step = 32 * (D + 2);
-  float top = -INF;
-  for (int n = 0; n < a.splits; ++n) top = fmaxf(top, p[n * step + D]);
-  const float base = top == -INF ? 0.f : top;
-  float z = 0.f, o = 0.f;
-  for (int n = 0; n < a.splits; ++n) {
-    const float f = __builtin_amdgcn_exp2f(p[n * step + D] - base);
-    z = fmaf(p[n * step + D + 1], f, z);
-    o = fmaf(p[n * step + threadIdx.x], f, o);
+  // every thread holds its column of up to 16 parts at a time, so that their
+  // loads are in flight together
+  float top = -INF, z = 0.f, o = 0.f;
+  for (int n0 = 0; n0 < a.splits; n0 += 16) {
+    float m[16], l[16], x[16], more = top;
+#pragma unroll
+    for (int n = 0; n < 16; ++n) {
+      const float* at_n = p + min(n0 + n, a.splits - 1) * step;
+      m[n] = n0 + n < a.splits ? at_n[D] : -INF;
+      l[n] = at_n[D + 1];
+      x[n] = at_n[threadIdx.x];
+    }
+#pragma unroll
+    for (int n = 0; n < 16; ++n) more = larger(more, m[n]);
+    const float base = more == -INF ? 0.f : more, f = __builtin_amdgcn_exp2f(top - base);
+    z *= f;
+    o *= f;
+    top = more;
+#pragma unroll
+    for (int n = 0; n < 16; ++n) {
+      const float g = __builtin_amdgcn_exp2f(m[n] - base);
+      z = fmaf(l[n], g, z);
+      o = fmaf(x[n], g, o);
+    }
   }
   a.out[(((long long)b * a.Sq + at / group) * a.NH + hk * group + at % group) * D + threadIdx.x] =
       (__bf16)(z == 0.f ? 0.f : o / z);

@@ -187,22 +187,39 @@ __device__ __forceinline__ float as_bias(__bf16 t, float scale) {
   return f < -3.38e38f ? -INF : f / scale;
 }
 
-__device__ __forceinline__ float bias_at(const RelArgs& a, int d, int h) {
-  const int n = min(max(a.map[d + a.far], 0), a.buckets - 1);
-  return as_bias(a.table[(long long)n * a.NH + h], a.scale);
-}
-
+// In two steps, so that the two dependent loads of an entry run beside the
+// kernel's other first loads: the constructor issues them, `put` stores.
 template <int T = 256>
-__device__ void stage_bias(const RelArgs& a, int h, int sign, float* bias) {
-  const int len = bias_len(a.far);
-  for (int x = threadIdx.x; x < len + 3; x += T) {
-    const int d = min(max(x - 7 - a.far, -a.far), a.far);
-    const float v = bias_at(a, sign * d, h);
+struct Bias {
+  static constexpr int N = (2 * GA_REL_MAX_DISTANCE + 17 + T - 1) / T;
+  __bf16 t[N];
+  int len;
+  __device__ __forceinline__ Bias(const RelArgs& a, int h, int sign) : len(bias_len(a.far)) {
+    int n[N];
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
-      if (x >= c && x - c < len) bias[c * len + x - c] = v;
+    for (int i = 0; i < N; ++i) {
+      if (i * T >= len + 3) break;
+      const int d = min(max((int)threadIdx.x + T * i - 7 - a.far, -a.far), a.far);
+      n[i] = a.map[sign * d + a.far];
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (i * T >= len + 3) break;
+      t[i] = a.table[(long long)min(max(n[i], 0), a.buckets - 1) * a.NH + h];
+    }
   }
-}
+  __device__ __forceinline__ void put(float scale, float* bias) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (i * T >= len + 3) break;
+      const float v = as_bias(t[i], scale);
+      const int x = threadIdx.x + T * i;
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        if (x >= c && x - c < len) bias[c * len + x - c] = v;
+    }
+  }
+};
 
 // C's initial value for rows u0 + crow(r) against column w: the bias of the
 // offset row - column. `low`, `high`: the values beyond the largest distance.
@@ -275,13 +292,16 @@ __device__ __forceinline__ bool key_on(const unsigned char* mask, int j0, int en
 
 // C rows whose key does not count, or lies behind the column's query -> fill
 __device__ __forceinline__ void drop_rows(f16& c, unsigned bits, bool diag, int key0, int query0, int lane, float fill) {
+  // the empty statements keep these branches: as selects they would run in every tile
   const int hi = lane >> 5;
   if (bits != ~0u) {
+    asm volatile("");
     const unsigned b = bits >> (4 * hi);
 #pragma unroll
     for (int r = 0; r < 16; ++r) c[r] = (b >> crow(r, 0)) & 1 ? c[r] : fill;
   }
   if (diag) {
+    asm volatile("");
     const int most = query0 + (lane & 31) - key0 - 4 * hi;
 #pragma unroll
     for (int r = 0; r < 16; ++r) c[r] = crow(r, 0) <= most ? c[r] : fill;
@@ -321,19 +341,9 @@ __global__ __launch_bounds__(256, 2) void k_rel_fwd(RelArgs a, int tiles) {
   const __bf16* v = k + a.NKV * D;
   const unsigned char* mask = a.mask ? a.mask + (long long)b * a.S : nullptr;
 
-  stage_bias(a, h, 1, bias);
   int end = a.causal ? min(a.S, tile * TILE + TILE) : a.S;
   if (mask) end = mask_end(mask, end, ends);
   const int chunks = (end + KC - 1) / KC;
-
-  b8 q[D / 16];
-  const __bf16* qp = a.qkv + ((long long)b * a.S + min(i, a.S - 1)) * a.width + h * D;
-#pragma unroll
-  for (int t = 0; t < D / 16; ++t) q[t] = *(const b8*)(qp + 16 * t + 8 * hi);
-
-  f16 o[D / 32] = {};
-  float m = -INF, l = 0.f;
-  const float c2 = a.scale * LOG2E;
 
   Stage<D> st;
   st.init(a.width, a.width);
@@ -350,12 +360,21 @@ __global__ __launch_bounds__(256, 2) void k_rel_fwd(RelArgs a, int tiles) {
     next = __ballot(key);
     st.clear(to, to + MAT, next);
   };
+  // everything that the first chunk needs is on its way at once
+  if (chunks > 0) fetch(0);
+  const Bias<> first_bias(a, h, 1);
+  b8 q[D / 16];
+  const __bf16* qp = a.qkv + ((long long)b * a.S + min(i, a.S - 1)) * a.width + h * D;
+#pragma unroll
+  for (int t = 0; t < D / 16; ++t) q[t] = *(const b8*)(qp + 16 * t + 8 * hi);
+  first_bias.put(a.scale, bias);
   st.wait();
-  if (chunks > 0) {
-    fetch(0);
-    arrive(0);
-  }
+  if (chunks > 0) arrive(0);
   __syncthreads();
+
+  f16 o[D / 32] = {};
+  float m = -INF, l = 0.f;
+  const float c2 = a.scale * LOG2E;
   const float low = bias[0], high = bias[2 * a.far + 7];
 
   for (int c = 0; c < chunks; ++c) {
@@ -442,6 +461,14 @@ __device__ __forceinline__ void diagonals(const f16& c, float* d) {
   if (s) d[u + 1] += from_lane<s ? s - 16 : 0>(c[R]);
   if constexpr (R < 15) diagonals<R + 1>(c, d);
 }
+// ... and the 16 columns of ib = 1 stand 16 offsets lower: with d[1] exchanged
+// between the two, d[0] and d[2] are the sums of 32 neighbouring offsets each.
+__device__ __forceinline__ void diagonals_32(const f16& c, float* d, bool ib) {
+  diagonals(c, d);
+  const float other = __builtin_bit_cast(float, __builtin_amdgcn_ds_swizzle(__builtin_bit_cast(int, d[1]), 0x401f));  // lane ^ 16
+  d[0] += ib ? 0.f : other;
+  d[2] += ib ? other : 0.f;
+}
 
 // ---------------- backward 1: dQ, D and the offsets' sums of dS ----------------
 template <int D>
@@ -464,12 +491,28 @@ __global__ __launch_bounds__(256, 2) void k_rel_bwd_q(RelArgs a, int tiles) {
   const __bf16* v = k + a.NKV * D;
   const unsigned char* mask = a.mask ? a.mask + (long long)b * a.S : nullptr;
 
-  stage_bias(a, h, 1, bias);
-  for (int x = threadIdx.x; x < 8 * offs; x += 256) sums[x] = 0.f;
   int end = a.causal ? min(a.S, tile * TILE + TILE) : a.S;
   if (mask) end = mask_end(mask, end, ends);
   const int chunks = (end + KC - 1) / KC;
 
+  Stage<D> st;
+  st.init(a.width, a.width);
+  unsigned long long bits = 0, next = 0;
+  bool key = false;
+  auto fetch = [&](int c) {
+    char* to = buf + (c & 1) * 2 * MAT;
+    key = key_on(mask, c * KC, end);
+    st.load(k, a.width, v, a.width, c * KC, end, to, to + MAT);
+  };
+  auto arrive = [&](int c) {
+    char* to = buf + (c & 1) * 2 * MAT;
+    st.wait();
+    next = __ballot(key);
+    st.clear(to, to + MAT, next);
+  };
+  // everything that the first chunk needs is on its way at once
+  if (chunks > 0) fetch(0);
+  const Bias<> first_bias(a, h, 1);
   // a row past the end, or with nothing allowed, takes part as zeros
   const float lse = i < a.S ? a.lse[(long long)bh * a.S + i] : INF;
   const bool live = lse < INF || lse != lse;
@@ -498,34 +541,23 @@ __global__ __launch_bounds__(256, 2) void k_rel_bwd_q(RelArgs a, int tiles) {
   const float c2 = a.scale * LOG2E;
   float* mine = sums + (2 * wave + hi) * offs;
   float far_low = 0.f, far_high = 0.f;
-  // diagonals not yet added: the last of a tile is the first of the next one
+  // The upper 32 offsets of a tile are the lower 32 of the next one: they wait in
+  // a register. What is added to LDS goes to the half wave's own array, 32 lanes
+  // to 32 offsets, so it needs no atomic (one costs as much as the tile's
+  // products); offsets beyond the largest distance, where lanes would meet, stay
+  // in registers.
   float left = 0.f;
-  int left_at = 0;
-  const int lane_off = 4 * hi - (lane & 31);  // 4 hi - 16 ib - i
+  int left_at = i0;  // the key tile that `left` is for
+  const int lane_off = 4 * hi - (lane & 31);
   auto add = [&](int d, float x) {
-    __hip_atomic_fetch_add(mine + min(max(d, -a.far), a.far) + a.far, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    far_low += d <= -a.far ? x : 0.f;
+    far_high += d >= a.far ? x : 0.f;
+    if (d > -a.far && d < a.far) mine[d + a.far] += x;
   };
-
-  Stage<D> st;
-  st.init(a.width, a.width);
-  unsigned long long bits = 0, next = 0;
-  bool key = false;
-  auto fetch = [&](int c) {
-    char* to = buf + (c & 1) * 2 * MAT;
-    key = key_on(mask, c * KC, end);
-    st.load(k, a.width, v, a.width, c * KC, end, to, to + MAT);
-  };
-  auto arrive = [&](int c) {
-    char* to = buf + (c & 1) * 2 * MAT;
-    st.wait();
-    next = __ballot(key);
-    st.clear(to, to + MAT, next);
-  };
+  first_bias.put(a.scale, bias);
+  for (int x = threadIdx.x; x < 8 * offs; x += 256) sums[x] = 0.f;
   st.wait();
-  if (chunks > 0) {
-    fetch(0);
-    arrive(0);
-  }
+  if (chunks > 0) arrive(0);
   __syncthreads();
   const float low = bias[0], high = bias[2 * a.far + 7];
 
@@ -535,27 +567,26 @@ __global__ __launch_bounds__(256, 2) void k_rel_bwd_q(RelArgs a, int tiles) {
     if (c + 1 < chunks) fetch(c + 1);
     const char* kt = buf + (c & 1) * 2 * MAT;
     const char* vt = kt + MAT;
-#pragma unroll
+#pragma unroll 1  // one copy of the code: on short sequences its fetches are what is waited for
     for (int sub = 0; sub < 2; ++sub) {
       const int j0 = c * KC + 32 * sub;
       const unsigned on = (unsigned)(bits >> (32 * sub));
       if (on == 0 || (a.causal && j0 > i0 + 31)) continue;
+      const char* ksub = kt + 64 * D * sub;
+      const char* vsub = vt + 64 * D * sub;
       f16 s = bias_tile(bias, a.far, j0, i0, lane, low, high);
       f16 dp = {};
 #pragma unroll
       for (int t = 0; t < D / 16; ++t) {
-        s = mfma(row_frag<D>(kt, 32 * sub + (lane & 31), t, hi), q[t], s);
-        dp = mfma(row_frag<D>(vt, 32 * sub + (lane & 31), t, hi), g[t], dp);
+        s = mfma(row_frag<D>(ksub, lane & 31, t, hi), q[t], s);
+        dp = mfma(row_frag<D>(vsub, lane & 31, t, hi), g[t], dp);
       }
       reads_ahead<D / 8>();
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c2, -lse)) * (dp[r] - dsum);
       drop_rows(s, on, a.causal && j0 + 31 > i0, j0, i0, lane, 0.f);
       // sums of dS by offset: tiles beyond the largest distance in a register,
-      // others along their diagonals, then by LDS additions into an array of
-      // this half wave's own (32 lanes, 32 offsets, no two at one address but
-      // where they are clamped; a wave's additions are made in order, so the
-      // result does not depend on timing)
+      // others along their diagonals
       if (j0 + 31 - i0 <= -a.far || j0 - (i0 + 31) >= a.far) {
         float t = 0.f;
 #pragma unroll
@@ -563,13 +594,11 @@ __global__ __launch_bounds__(256, 2) void k_rel_bwd_q(RelArgs a, int tiles) {
         if (j0 < i0) far_low += t;
         else far_high += t;
       } else {
-        const int d0 = j0 - i0 + lane_off;
         float d[3] = {};
-        if (left_at == j0) d[0] = left;
-        else add(left_at - i0 + lane_off, left);
-        diagonals(s, d);
-        add(d0, d[0]);
-        add(d0 + 16, d[1]);
+        if (left_at != j0) add(left_at - i0 + lane_off, left);
+        else d[0] = left;
+        diagonals_32(s, d, lane & 16);
+        add(j0 - i0 + lane_off, d[0]);
         left = d[2];
         left_at = j0 + 32;
       }
@@ -577,7 +606,7 @@ __global__ __launch_bounds__(256, 2) void k_rel_bwd_q(RelArgs a, int tiles) {
       for (int ks = 0; ks < 2; ++ks) {
         const b8 p = pack(s, ks);
 #pragma unroll
-        for (int dt = 0; dt < D / 32; ++dt) dq[dt] = mfma(col_frag<D>(kt, 32 * sub + 16 * ks, dt, lane), p, dq[dt]);
+        for (int dt = 0; dt < D / 32; ++dt) dq[dt] = mfma(col_frag<D>(ksub, 16 * ks, dt, lane), p, dq[dt]);
       }
     }
     if (c + 1 < chunks) arrive(c + 1);
@@ -678,8 +707,8 @@ __global__ __launch_bounds__(SPLIT ? 512 : 256, 2) void k_rel_bwd_kv(RelArgs a, 
         }
       };
       __syncthreads();  // the last head's tiles are read
-      stage_bias<T>(a, h, -1, bias);
       fetch(first);
+      Bias<T>(a, h, -1).put(a.scale, bias);
       put(first);
       __syncthreads();
       const float low = bias[0], high = bias[2 * a.far + 7];
@@ -715,6 +744,7 @@ __global__ __launch_bounds__(SPLIT ? 512 : 256, 2) void k_rel_bwd_kv(RelArgs a, 
             reads_ahead<D / 8>();
           }
           if (a.causal && i0 < j0 + 31) {
+            asm volatile("");
             const int least = j - i0 - 4 * hi;
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[r] = crow(r, 0) >= least ? s[r] : -INF;

@@ -175,7 +175,7 @@ struct Stage {
 };
 
 // ---- the bias of one head in LDS: entry x is the offset clamp(x - 7 - far),
-// copy c holds the entries from c on. `sign` -1: offsets mirrored.
+// copy c holds the entries from c on.
 __host__ __device__ __forceinline__ int bias_top(int far) { return (2 * far + 10) & ~3; }  // from here on all are the last offset's
 __host__ __device__ __forceinline__ int bias_len(int far) { return bias_top(far) + 4; }
 
@@ -187,20 +187,26 @@ __device__ __forceinline__ float as_bias(__bf16 t, float scale) {
   return f < -3.38e38f ? -INF : f / scale;
 }
 
+__device__ __forceinline__ void put_bias(float* bias, int len, int x, float v) {
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    if (x >= c && x - c < len) bias[c * len + x - c] = v;
+}
+
 // In two steps, so that the two dependent loads of an entry run beside the
 // kernel's other first loads: the constructor issues them, `put` stores.
-template <int T = 256>
 struct Bias {
+  static constexpr int T = 256;
   static constexpr int N = (2 * GA_REL_MAX_DISTANCE + 17 + T - 1) / T;
   __bf16 t[N];
   int len;
-  __device__ __forceinline__ Bias(const RelArgs& a, int h, int sign) : len(bias_len(a.far)) {
+  __device__ __forceinline__ Bias(const RelArgs& a, int h) : len(bias_len(a.far)) {
     int n[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       if (i * T >= len + 3) break;
       const int d = min(max((int)threadIdx.x + T * i - 7 - a.far, -a.far), a.far);
-      n[i] = a.map[sign * d + a.far];
+      n[i] = a.map[d + a.far];
     }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -212,11 +218,7 @@ struct Bias {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       if (i * T >= len + 3) break;
-      const float v = as_bias(t[i], scale);
-      const int x = threadIdx.x + T * i;
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-        if (x >= c && x - c < len) bias[c * len + x - c] = v;
+      put_bias(bias, len, threadIdx.x + T * i, as_bias(t[i], scale));
     }
   }
 };
@@ -362,7 +364,7 @@ __global__ __launch_bounds__(256, 2) void k_rel_fwd(RelArgs a, int tiles) {
   };
   // everything that the first chunk needs is on its way at once
   if (chunks > 0) fetch(0);
-  const Bias<> first_bias(a, h, 1);
+  const Bias first_bias(a, h);
   b8 q[D / 16];
   const __bf16* qp = a.qkv + ((long long)b * a.S + min(i, a.S - 1)) * a.width + h * D;
 #pragma unroll
@@ -512,7 +514,7 @@ __global__ __launch_bounds__(256, 2) void k_rel_bwd_q(RelArgs a, int tiles) {
   };
   // everything that the first chunk needs is on its way at once
   if (chunks > 0) fetch(0);
-  const Bias<> first_bias(a, h, 1);
+  const Bias first_bias(a, h);
   // a row past the end, or with nothing allowed, takes part as zeros
   const float lse = i < a.S ? a.lse[(long long)bh * a.S + i] : INF;
   const bool live = lse < INF || lse != lse;
@@ -541,6 +543,12 @@ __global__ __launch_bounds__(256, 2) void k_rel_bwd_q(RelArgs a, int tiles) {
   const float c2 = a.scale * LOG2E;
   float* mine = sums + (2 * wave + hi) * offs;
   float far_low = 0.f, far_high = 0.f;
+  // This row's dS must sum to zero. It does not quite: D comes from out as it was
+  // rounded, and what D is off by goes into a bucket with the bucket's share of P.
+  // In one that holds most of P but sums to little (all keys beyond the largest
+  // distance of a long sequence) that would be most of the result; so the row's
+  // sum `rest` is taken out of the two outermost offsets by their share of P.
+  float rest = 0.f, own_low = 0.f, own_high = 0.f, mass_low = 0.f, mass_high = 0.f;
   // The upper 32 offsets of a tile are the lower 32 of the next one: they wait in
   // a register. What is added to LDS goes to the half wave's own array, 32 lanes
   // to 32 offsets, so it needs no atomic (one costs as much as the tile's
@@ -583,28 +591,38 @@ __global__ __launch_bounds__(256, 2) void k_rel_bwd_q(RelArgs a, int tiles) {
       }
       reads_ahead<D / 8>();
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c2, -lse)) * (dp[r] - dsum);
+      for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c2, -lse));
       drop_rows(s, on, a.causal && j0 + 31 > i0, j0, i0, lane, 0.f);
+      float whole = 0.f;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        dp[r] = s[r] * (dp[r] - dsum);
+        whole += dp[r];
+      }
       // sums of dS by offset: tiles beyond the largest distance in a register,
       // others along their diagonals
+      rest += whole;
       if (j0 + 31 - i0 <= -a.far || j0 - (i0 + 31) >= a.far) {
         float t = 0.f;
 #pragma unroll
         for (int r = 0; r < 16; ++r) t += s[r];
-        if (j0 < i0) far_low += t;
-        else far_high += t;
+        const bool low_side = j0 < i0;
+        own_low += low_side ? whole : 0.f;
+        own_high += low_side ? 0.f : whole;
+        mass_low += low_side ? t : 0.f;
+        mass_high += low_side ? 0.f : t;
       } else {
         float d[3] = {};
         if (left_at != j0) add(left_at - i0 + lane_off, left);
         else d[0] = left;
-        diagonals_32(s, d, lane & 16);
+        diagonals_32(dp, d, lane & 16);
         add(j0 - i0 + lane_off, d[0]);
         left = d[2];
         left_at = j0 + 32;
       }
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks) {
-        const b8 p = pack(s, ks);
+        const b8 p = pack(dp, ks);
 #pragma unroll
         for (int dt = 0; dt < D / 32; ++dt) dq[dt] = mfma(col_frag<D>(ksub, 16 * ks, dt, lane), p, dq[dt]);
       }
@@ -614,6 +632,9 @@ __global__ __launch_bounds__(256, 2) void k_rel_bwd_q(RelArgs a, int tiles) {
   if (i < a.S)
     store_columns<D>(a.dqkv + ((long long)b * a.S + i) * a.width + h * D, dq, a.scale, hi);
   add(left_at - i0 + lane_off, left);
+  rest += __shfl_xor(rest, 32, 64);
+  far_low += fmaf(-rest, mass_low, own_low);  // each half takes its own share
+  far_high += fmaf(-rest, mass_high, own_high);
 #pragma unroll
   for (int x = 32; x > 0; x >>= 1) {
     far_low += __shfl_xor(far_low, x, 64);
@@ -634,32 +655,35 @@ __global__ __launch_bounds__(256, 2) void k_rel_bwd_q(RelArgs a, int tiles) {
 }
 
 // ---------------- backward 2: dK and dV; a wave owns 32 keys, chunks of 64 queries ----------------
-// SPLIT (head size 128): dK, dV, K and V of 32 keys fill a wave's registers, one
-// wave a SIMD is left, and products and exponentials wait for each other. So two
-// waves share the keys: the first four make dV, the other four dK. Both compute
-// the scores (40 matrix instructions a tile instead of 32), but two waves a SIMD
-// run side by side: MEASURED
-template <int D, bool SPLIT>
-__global__ __launch_bounds__(SPLIT ? 512 : 256, 2) void k_rel_bwd_kv(RelArgs a, int tiles) {
-  constexpr int T = SPLIT ? 512 : 256;
-  extern __shared__ __align__(16) char smem[];  // the tiles lie in the first 64 KB, which m0 reaches
+// Registers decide here: dK, dV, K and V of 32 keys are 256 of them at head size
+// 128. V is kept in LDS there, by eight waves that share a chunk instead of four:
+// two waves a SIMD. Measured at 2x4093 causal, 16 heads over 4, D 128: 480 us
+// with V in registers, 325 us so; at 16x512, 12 heads, D 64: 45 us with V in
+// registers, 61 us in LDS with four waves, 85 us with eight.
+template <int D>
+constexpr int kv_waves() { return D == 64 ? 4 : 8; }
+template <int D>
+__global__ __launch_bounds__(64 * kv_waves<D>(), D == 64 ? 3 : 2) void k_rel_bwd_kv(RelArgs a, int tiles) {
+  constexpr int T = 64 * kv_waves<D>(), KEYS = T / 2;
+  constexpr bool V_LDS = D == 128;
+  extern __shared__ __align__(16) char smem[];  // the chunks lie in the first 64 KB, which m0 reaches
   char* buf = smem;                             // [2][Q, dO]
   constexpr int MAT = KC * 2 * D;
-  float* rows = (float*)(smem + 4 * MAT);  // [2][lse, D][64]
-  float* bias = rows + 4 * KC;
+  float* rows = (float*)(smem + 4 * MAT);    // [2][lse, D][64]
+  char* vt = (char*)(rows + 4 * KC);         // V_LDS: [KEYS][D]
+  float* bias = (float*)(vt + (V_LDS ? KEYS * 2 * D : 0));
 
   int tile;
   const int column = place(a.B * a.NKV, a.parts, tiles, a.causal, tile);  // the first tile has the most queries
   const int part = column % a.parts, bk = column / a.parts;
   const int hk = bk % a.NKV, b = bk / a.NKV, group = a.NH / a.NKV;
   const int lane = threadIdx.x & 63, hi = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const bool for_k = SPLIT && wave >= 4;
-  const int j0 = tile * TILE + (wave & 3) * 32, j = j0 + (lane & 31);
+  const int row = (threadIdx.x >> 6) * 32 + (lane & 31);  // of the tile's keys
+  const int j0 = tile * KEYS + (threadIdx.x >> 6) * 32, j = j0 + (lane & 31);
   const bool keep = j < a.S && (!a.mask || a.mask[(long long)b * a.S + min(j, a.S - 1)]);
   const bool work = __any(keep);  // this wave has a key that counts
 
-  b8 k[D / 16], v[D / 16];
+  b8 k[D / 16], v[V_LDS ? 1 : D / 16];
   {
     const int r = min(j, a.S - 1);
     const __bf16* kp = a.qkv + ((long long)b * a.S + r) * a.width + (a.NH + hk) * D;
@@ -668,14 +692,15 @@ __global__ __launch_bounds__(SPLIT ? 512 : 256, 2) void k_rel_bwd_kv(RelArgs a, 
 #pragma unroll
     for (int t = 0; t < D / 16; ++t) {
       k[t] = *(const b8*)(kp + 16 * t + 8 * hi);
-      v[t] = *(const b8*)(vp + 16 * t + 8 * hi);
+      const b8 x = *(const b8*)(vp + 16 * t + 8 * hi);
       k[t] = keep ? k[t] : zero;
-      v[t] = keep ? v[t] : zero;
+      if (V_LDS) *(b8*)(vt + piece<D>(row, 2 * t + hi)) = keep ? x : zero;  // read by this wave alone
+      else v[V_LDS ? 0 : t] = keep ? x : zero;
     }
   }
-  f16 acc[D / 32] = {}, dv[SPLIT ? 1 : D / 32] = {};  // dK (SPLIT: dK or dV), dV
+  f16 dk[D / 32] = {}, dv[D / 32] = {};
   const float c2 = a.scale * LOG2E;
-  const int first = a.causal ? tile * TILE / KC : 0, chunks = (a.S + KC - 1) / KC;
+  const int first = a.causal ? tile * KEYS / KC : 0, chunks = (a.S + KC - 1) / KC;
   Stage<D, T> st;
   st.init(a.width, a.NH * D);
   float row_lse = 0.f, row_d = 0.f;
@@ -708,7 +733,13 @@ __global__ __launch_bounds__(SPLIT ? 512 : 256, 2) void k_rel_bwd_kv(RelArgs a, 
       };
       __syncthreads();  // the last head's tiles are read
       fetch(first);
-      Bias<T>(a, h, -1).put(a.scale, bias);
+      // (in a plain loop: this kernel has no register to spare)
+#pragma unroll 1
+      for (int x = threadIdx.x; x < bias_len(a.far) + 3; x += T) {
+        const int d = min(max(a.far + 7 - x, -a.far), a.far);  // mirrored
+        const int at = min(max(a.map[d + a.far], 0), a.buckets - 1);
+        put_bias(bias, bias_len(a.far), x, as_bias(a.table[(long long)at * a.NH + h], a.scale));
+      }
       put(first);
       __syncthreads();
       const float low = bias[0], high = bias[2 * a.far + 7];
@@ -726,23 +757,12 @@ __global__ __launch_bounds__(SPLIT ? 512 : 256, 2) void k_rel_bwd_kv(RelArgs a, 
           const char* gs = gt + 64 * D * sub;
           // rows are queries here: the mirrored bias of row - column
           f16 s = bias_tile(bias, a.far, i0, j0, lane, low, high), dp = {};
-          if (SPLIT) {
 #pragma unroll
-            for (int t = 0; t < D / 16; ++t) s = mfma(row_frag<D>(qs, lane & 31, t, hi), k[t], s);
-            reads_ahead<D / 16>();
-            if (for_k) {
-#pragma unroll
-              for (int t = 0; t < D / 16; ++t) dp = mfma(row_frag<D>(gs, lane & 31, t, hi), v[t], dp);
-              reads_ahead<D / 16>();
-            }
-          } else {
-#pragma unroll
-            for (int t = 0; t < D / 16; ++t) {
-              s = mfma(row_frag<D>(qs, lane & 31, t, hi), k[t], s);
-              dp = mfma(row_frag<D>(gs, lane & 31, t, hi), v[t], dp);
-            }
-            reads_ahead<D / 8>();
+          for (int t = 0; t < D / 16; ++t) {
+            s = mfma(row_frag<D>(qs, lane & 31, t, hi), k[t], s);
+            dp = mfma(row_frag<D>(gs, lane & 31, t, hi), V_LDS ? row_frag<D>(vt, row, t, hi) : v[V_LDS ? 0 : t], dp);
           }
+          if (!V_LDS) reads_ahead<D / 8>();
           if (a.causal && i0 < j0 + 31) {
             asm volatile("");
             const int least = j - i0 - 4 * hi;
@@ -755,31 +775,19 @@ __global__ __launch_bounds__(SPLIT ? 512 : 256, 2) void k_rel_bwd_kv(RelArgs a, 
 #pragma unroll
             for (int y = 0; y < 4; ++y) s[4 * x + y] = __builtin_amdgcn_exp2f(fmaf(s[4 * x + y], c2, -e[y]));
           }
-          if (!SPLIT || for_k)
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              const f4 d = *(const f4*)(rl + KC + 32 * sub + 8 * x + 4 * hi);
+          for (int x = 0; x < 4; ++x) {
+            const f4 d = *(const f4*)(rl + KC + 32 * sub + 8 * x + 4 * hi);
 #pragma unroll
-              for (int y = 0; y < 4; ++y) dp[4 * x + y] = (dp[4 * x + y] - d[y]) * s[4 * x + y];
-            }
-          if (SPLIT) {
-            const char* from = for_k ? qs : gs;
-            if (for_k) s = dp;
+            for (int y = 0; y < 4; ++y) dp[4 * x + y] = (dp[4 * x + y] - d[y]) * s[4 * x + y];
+          }
 #pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
-              const b8 p = pack(s, ks);
+          for (int ks = 0; ks < 2; ++ks) {
+            const b8 p = pack(s, ks), ds = pack(dp, ks);
 #pragma unroll
-              for (int dt = 0; dt < D / 32; ++dt) acc[dt] = mfma(col_frag<D>(from, 16 * ks, dt, lane), p, acc[dt]);
-            }
-          } else {
-#pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
-              const b8 p = pack(s, ks), ds = pack(dp, ks);
-#pragma unroll
-              for (int dt = 0; dt < D / 32; ++dt) {
-                dv[SPLIT ? 0 : dt] = mfma(col_frag<D>(gs, 16 * ks, dt, lane), p, dv[SPLIT ? 0 : dt]);
-                acc[dt] = mfma(col_frag<D>(qs, 16 * ks, dt, lane), ds, acc[dt]);
-              }
+            for (int dt = 0; dt < D / 32; ++dt) {
+              dv[dt] = mfma(col_frag<D>(gs, 16 * ks, dt, lane), p, dv[dt]);
+              dk[dt] = mfma(col_frag<D>(qs, 16 * ks, dt, lane), ds, dk[dt]);
             }
           }
         }
@@ -790,8 +798,8 @@ __global__ __launch_bounds__(SPLIT ? 512 : 256, 2) void k_rel_bwd_kv(RelArgs a, 
   // a masked key's column holds what its zeroed K and V gave: it has no gradient
   const f16 none[D / 32] = {};
   auto write = [&](auto* at, int step) {
-    if (!SPLIT || for_k) store_columns<D>(at, keep ? acc : none, a.scale, hi);
-    if (SPLIT ? !for_k : true) store_columns<D>(at + step, keep ? (SPLIT ? acc : dv) : none, 1.f, hi);
+    store_columns<D>(at, keep ? dk : none, a.scale, hi);
+    store_columns<D>(at + step, keep ? dv : none, 1.f, hi);
   };
   if (a.parts > 1) write(a.dkv + (((long long)part * a.B * a.NKV + bk) * a.S + j) * 2 * D, D);
   else write(a.dqkv + ((long long)b * a.S + j) * a.width + (a.NH + hk) * D, a.NKV * D);
@@ -1084,14 +1092,15 @@ template <int D>
 hipError_t backward(const RelArgs& a, hipStream_t s) {
   const int tiles = rel_tiles(a.S);
   const size_t lds_q = 4 * KC * 2 * D + bias_bytes(a.far) + 16 + 32 * (2 * a.far + 1);
-  const size_t lds_kv = 4 * KC * 2 * D + 16 * KC + bias_bytes(a.far);
+  constexpr int T = 64 * kv_waves<D>();
+  const int kv_tiles = (a.S + T / 2 - 1) / (T / 2);
+  const size_t lds_kv = 4 * KC * 2 * D + 16 * KC + (D == 128 ? T * D : 0) + bias_bytes(a.far);
   hipError_t e = allow(k_rel_bwd_q<D>, lds_q);
-  constexpr bool SPLIT = D == 128;
-  if (e == hipSuccess) e = allow(k_rel_bwd_kv<D, SPLIT>, lds_kv);
+  if (e == hipSuccess) e = allow(k_rel_bwd_kv<D>, lds_kv);
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL((k_rel_bwd_q<D>), dim3(a.B * a.NH * tiles), dim3(256), lds_q, s, a, tiles);
   if ((e = hipGetLastError()) != hipSuccess) return e;
-  hipLaunchKernelGGL((k_rel_bwd_kv<D, SPLIT>), dim3(a.B * a.NKV * a.parts * tiles), dim3(SPLIT ? 512 : 256), lds_kv, s, a, tiles);
+  hipLaunchKernelGGL((k_rel_bwd_kv<D>), dim3(a.B * a.NKV * a.parts * kv_tiles), dim3(T), lds_kv, s, a, kv_tiles);
   if ((e = hipGetLastError()) != hipSuccess) return e;
   if (a.parts > 1) {
     const long long n = (long long)a.B * a.NKV * a.S * (D / 2);

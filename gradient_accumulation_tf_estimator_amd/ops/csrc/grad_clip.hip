@@ -126,7 +126,7 @@ __device__ void scale(const E* in, E* out, long long n, float c, bool vec) {
       for (int k = 0; k < 4; ++k) {
 #pragma unroll
         for (int e = 0; e < V; ++e) v[k][e] = (E)((float)v[k][e] * c);
-        o[i + 256 * k] = v[k];
+        __builtin_nontemporal_store(v[k], o + i + 256 * k);
       }
     }
     for (; i < nv; i += 256) {
@@ -140,11 +140,14 @@ __device__ void scale(const E* in, E* out, long long n, float c, bool vec) {
   for (; i < n; i += 256) out[i] = (E)((float)in[i] * c);
 }
 
+// Blocks run from the last chunk to the first: what the norm's pass read last is
+// still in the 256 MB cache (335M fp32 elements, 1.3 GB: 852 -> 839 us in all, 802 us
+// with stores that do not push it out).
 __global__ __launch_bounds__(256) void k_clip_scale(ClipArgs a, const float* coef) {
   const float c = *coef;
-  const int t = tensor_of(a, blockIdx.x);
+  const int b = gridDim.x - 1 - blockIdx.x, t = tensor_of(a, b);
   if (c == 1.f && a.in[t] == a.out[t]) return;  // in place and nothing to clip
-  const long long at = (long long)(blockIdx.x - a.first[t]) * a.chunk;
+  const long long at = (long long)(b - a.first[t]) * a.chunk;
   const long long left = a.n[t] - at, n = left < a.chunk ? left : a.chunk;
   if (a.type[t] == GA_FP32) scale((const float*)a.in[t] + at, (float*)a.out[t] + at, n, c, a.vec[t]);
   else if (a.type[t] == GA_BF16) scale((const __bf16*)a.in[t] + at, (__bf16*)a.out[t] + at, n, c, a.vec[t]);

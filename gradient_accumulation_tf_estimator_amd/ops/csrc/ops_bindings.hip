@@ -286,7 +286,7 @@ std::tuple<at::Tensor, std::vector<at::Tensor>> global_norm(std::vector<at::Tens
   check_launch(clip_finish(blocks ? sums.data_ptr<double>() : nullptr, (int)blocks, clip, r, write ? r + 1 : nullptr, s),
                "global_norm");
   if (write)
-    for (const auto& a : launches) check_launch(clip_scale(a, r + 1, s), "clip_by_global_norm");
+    for (size_t i = launches.size(); i-- > 0;) check_launch(clip_scale(launches[i], r + 1, s), "clip_by_global_norm");
   return {result.select(0, 0), outs};
 }
 

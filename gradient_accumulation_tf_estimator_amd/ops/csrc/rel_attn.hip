@@ -829,7 +829,9 @@ __global__ __launch_bounds__(256) void k_rel_dkv(RelArgs a, long long n) {
 __global__ __launch_bounds__(1024) void k_rel_dtable(RelArgs a, int tiles) {
   __shared__ float part[16][320];
   __shared__ float sums[2 * GA_REL_MAX_DISTANCE + 1];
+  __shared__ short map[2 * GA_REL_MAX_DISTANCE + 1];
   const int h = blockIdx.x, offs = 2 * a.far + 1, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int x = threadIdx.x; x < offs; x += 1024) map[x] = (short)min(max(a.map[x], 0), a.buckets - 1);
   const int n = a.B * tiles;
   const float* p = a.doff + (long long)h * n * offs;
   for (int x0 = 0; x0 < offs; x0 += 320) {
@@ -853,7 +855,7 @@ __global__ __launch_bounds__(1024) void k_rel_dtable(RelArgs a, int tiles) {
   for (int bucket = wave; bucket < a.buckets; bucket += 16) {
     float t = 0.f;
     for (int e = lane; e < offs; e += 64)
-      if (min(max(a.map[e], 0), a.buckets - 1) == bucket) t += sums[e];
+      if (map[e] == bucket) t += sums[e];
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) t += __shfl_xor(t, o, 64);
     if (lane == 0) a.dtable[(long long)bucket * a.NH + h] = (__bf16)t;

@@ -29,11 +29,15 @@ if __name__ == "__main__":
     p.add_argument("--accum", type=int, default=4)
     p.add_argument("--lr", type=float, default=2e-5)
     p.add_argument("--warmup", type=int, default=100)
+    p.add_argument("--relative-buckets", type=int, default=0,
+                   help="buckets of a learned relative position bias (0: none)")
+    p.add_argument("--norm", choices=("layer", "rms"), default="layer")
     args = p.parse_args()
 
     ctx = init_distributed()
     torch.manual_seed(19830610 + ctx.rank)
     cfg = CONFIGS[args.model]()
+    cfg.relative_buckets, cfg.norm = args.relative_buckets, args.norm
     dtype = torch.bfloat16 if ctx.device.type == "cuda" else torch.float32
     model = BertForSequenceClassification(cfg).to(ctx.device, dtype)
 

@@ -37,6 +37,8 @@ from ..ops.fused import (
     fused_attention,
     fused_attention_supported,
 )
+from ..ops.relative_attention import RelativePositionBias
+from ..ops.rms_norm import FusedAddRMSNorm
 
 
 @dataclass
@@ -53,6 +55,11 @@ class BertConfig:
     num_labels: int = 2
     initializer_range: float = 0.02
     fused: bool = True  # use the fused LN/GELU HIP modules (A/B switch)
+    # a learned bias by relative position, shared by the layers (0: none); on a
+    # GPU it needs bf16, head size 64 or 128 and dropout 0
+    relative_buckets: int = 0
+    relative_max_distance: int = 128
+    norm: str = "layer"  # "rms": root-mean-square norms, projections without biases
 
 
 # BASELINE.json model configs
@@ -71,6 +78,16 @@ def bert_large() -> BertConfig:
 CONFIGS = {"bert-small": bert_small, "bert-base": bert_base, "bert-large": bert_large}
 
 
+def _norm(cfg: BertConfig, proj_bias: bool = False) -> nn.Module:
+    if cfg.norm == "rms":
+        return FusedAddRMSNorm(cfg.hidden_size, eps=cfg.layer_norm_eps)
+    if cfg.norm != "layer":
+        raise ValueError(f"norm must be 'layer' or 'rms', got {cfg.norm!r}")
+    if cfg.fused:
+        return FusedAddLayerNorm(cfg.hidden_size, eps=cfg.layer_norm_eps, proj_bias=proj_bias)
+    return nn.LayerNorm(cfg.hidden_size, eps=cfg.layer_norm_eps)
+
+
 class BertEmbeddings(nn.Module):
     def __init__(self, cfg: BertConfig):
         super().__init__()
@@ -78,8 +95,7 @@ class BertEmbeddings(nn.Module):
         self.word_embeddings = Emb(cfg.vocab_size, cfg.hidden_size)
         self.position_embeddings = Emb(cfg.max_position_embeddings, cfg.hidden_size)
         self.token_type_embeddings = Emb(cfg.type_vocab_size, cfg.hidden_size)
-        self.LayerNorm = (FusedAddLayerNorm(cfg.hidden_size, eps=cfg.layer_norm_eps)
-                          if cfg.fused else nn.LayerNorm(cfg.hidden_size, eps=cfg.layer_norm_eps))
+        self.LayerNorm = _norm(cfg)
         self.dropout = nn.Dropout(cfg.dropout)
         self.register_buffer(
             "position_ids", torch.arange(cfg.max_position_embeddings).unsqueeze(0), persistent=False
@@ -121,9 +137,11 @@ class BertSelfAttention(nn.Module):
         self.qkv = Lin(cfg.hidden_size, 3 * cfg.hidden_size)
         self.dropout_p = cfg.dropout
 
-    def forward(self, x, attn_mask=None, mask8=None, seed=None):
+    def forward(self, x, attn_mask=None, mask8=None, seed=None, relative=None):
         B, S, H = x.shape
         qkv = self.qkv(x)  # [B, S, 3H]
+        if relative is not None:
+            return relative(qkv, mask8=mask8)
         dp = self.dropout_p if self.training else 0.0
         if (x.is_cuda and x.dtype == torch.bfloat16 and self.head_dim == 64
                 and (dp == 0.0 or seed is not None)
@@ -156,10 +174,11 @@ class BertLayer(nn.Module):
         self.fused = cfg.fused
         Lin = DirectLinear if cfg.fused else nn.Linear
         self.attention = BertSelfAttention(cfg)
-        self.attention_output = Lin(cfg.hidden_size, cfg.hidden_size, bias=not cfg.fused)
+        out_bias = not cfg.fused and cfg.norm != "rms"
+        self.attention_output = Lin(cfg.hidden_size, cfg.hidden_size, bias=out_bias)
         if not cfg.fused:
             self.intermediate = nn.Linear(cfg.hidden_size, cfg.intermediate_size)
-            self.output = nn.Linear(cfg.intermediate_size, cfg.hidden_size)
+            self.output = nn.Linear(cfg.intermediate_size, cfg.hidden_size, bias=out_bias)
         self.dropout = nn.Dropout(cfg.dropout)
         # GA_CUSTOM_FFN: "1" force, "0" off, "auto" (default) = on for the
         # shapes where the k_ffn_* MFMA-epilogue kernels measured faster
@@ -175,8 +194,7 @@ class BertLayer(nn.Module):
                             and ffn_mfma_supported(cfg.hidden_size,
                                                    cfg.intermediate_size))
         if cfg.fused:
-            self.attention_LayerNorm = FusedAddLayerNorm(
-                cfg.hidden_size, eps=cfg.layer_norm_eps, proj_bias=True)
+            self.attention_LayerNorm = _norm(cfg, proj_bias=True)
             if self._custom_ffn:
                 # GA_CUSTOM_FFN=1: both FFN boundary GEMMs with the GELU in
                 # the MFMA epilogue (ops/csrc/ffn_mfma.hip) -- no standalone
@@ -193,11 +211,10 @@ class BertLayer(nn.Module):
                 self.intermediate_act = FusedBiasGelu(cfg.intermediate_size)
                 self.output = DirectLinear(cfg.intermediate_size,
                                            cfg.hidden_size, bias=False)
-            self.output_LayerNorm = FusedAddLayerNorm(
-                cfg.hidden_size, eps=cfg.layer_norm_eps, proj_bias=True)
+            self.output_LayerNorm = _norm(cfg, proj_bias=True)
         else:
-            self.attention_LayerNorm = nn.LayerNorm(cfg.hidden_size, eps=cfg.layer_norm_eps)
-            self.output_LayerNorm = nn.LayerNorm(cfg.hidden_size, eps=cfg.layer_norm_eps)
+            self.attention_LayerNorm = _norm(cfg)
+            self.output_LayerNorm = _norm(cfg)
 
     def _load_from_state_dict(self, state_dict, prefix, *args, **kw):
         # checkpoints are loadable across the GA_CUSTOM_FFN setting: the
@@ -215,11 +232,14 @@ class BertLayer(nn.Module):
     def _bind_direct_extras(self, engine):
         # the intermediate Linear's wgrad colsum over d(pre-gelu) IS the
         # gelu bias gradient: delegate it so gelu backward is elementwise
+        # (the RMS norm hands its residual's gradient on by itself)
+        defer = isinstance(self.attention_LayerNorm, FusedAddLayerNorm)
         if self.fused and self._custom_ffn:
             # FusedFFN owns its bias-grad wgrad entry; only the deferred
             # residual grad needs wiring (rides the FFN dx dgrad epilogue)
-            self.attention_LayerNorm._defer_residual_to = self.attention.qkv
-            self.output_LayerNorm._defer_residual_to = self.ffn
+            if defer:
+                self.attention_LayerNorm._defer_residual_to = self.attention.qkv
+                self.output_LayerNorm._defer_residual_to = self.ffn
             return
         if self.fused:
             self.intermediate._accum_view_b = engine.state.accum_view(
@@ -231,11 +251,12 @@ class BertLayer(nn.Module):
             # output_LayerNorm's dres rides intermediate's dgrad. Ordering:
             # the LN backward runs strictly before that dgrad, and the
             # summed grad's consumers run strictly after it.
-            self.attention_LayerNorm._defer_residual_to = self.attention.qkv
-            self.output_LayerNorm._defer_residual_to = self.intermediate
+            if defer:
+                self.attention_LayerNorm._defer_residual_to = self.attention.qkv
+                self.output_LayerNorm._defer_residual_to = self.intermediate
 
-    def forward(self, x, attn_mask=None, mask8=None, seed=None):
-        a = self.attention(x, attn_mask, mask8=mask8, seed=seed)
+    def forward(self, x, attn_mask=None, mask8=None, seed=None, relative=None):
+        a = self.attention(x, attn_mask, mask8=mask8, seed=seed, relative=relative)
         if self.fused:
             x = self.attention_LayerNorm(self.dropout(self.attention_output(a)), residual=x)
             if self._custom_ffn:
@@ -254,6 +275,12 @@ class BertModel(nn.Module):
         self.cfg = cfg
         self.embeddings = BertEmbeddings(cfg)
         self.encoder = nn.ModuleList(BertLayer(cfg) for _ in range(cfg.num_layers))
+        self.relative_attention_bias = None
+        if cfg.relative_buckets:
+            if cfg.dropout:
+                raise ValueError("relative_buckets needs dropout 0: relative attention has no dropout")
+            self.relative_attention_bias = RelativePositionBias(
+                cfg.num_heads, cfg.relative_buckets, cfg.relative_max_distance)
         self.pooler = (DirectLinear if cfg.fused else nn.Linear)(
             cfg.hidden_size, cfg.hidden_size)
         # per-layer attention-dropout seeds; refreshed each training forward
@@ -286,7 +313,8 @@ class BertModel(nn.Module):
         x = self.embeddings(input_ids, token_type_ids)
         for i, layer in enumerate(self.encoder):
             x = layer(x, mask, mask8=mask8,
-                      seed=None if seeds is None else seeds[i])
+                      seed=None if seeds is None else seeds[i],
+                      relative=self.relative_attention_bias)
         # pre-tanh pooler output; the tanh lives in the head (fused CE path)
         return x, self.pooler(x[:, 0])
 

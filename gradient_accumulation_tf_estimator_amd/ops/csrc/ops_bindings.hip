@@ -71,12 +71,13 @@ RmsArgs norm_args(const at::Tensor& x, const at::Tensor& w, double eps, bool& ve
   return a;
 }
 
-std::vector<at::Tensor> rms_norm_fwd(at::Tensor x, MaybeTensor res, at::Tensor w, double eps) {
+// x, res: rows; the outputs have the caller's shape, so that none is a view
+std::vector<at::Tensor> rms_norm_fwd(at::Tensor x, MaybeTensor res, at::Tensor w, double eps, at::IntArrayRef shape) {
   bool vec;
   RmsArgs a = norm_args(x, w, eps, vec);
   const c10::OptionalDeviceGuard guard(x.device());
-  auto y = at::empty({x.size(0), x.size(1)}, x.options());
-  auto h = res ? at::empty({x.size(0), x.size(1)}, x.options()) : x;
+  auto y = at::empty(shape, x.options());
+  auto h = res ? at::empty(shape, x.options()) : x;
   auto rstd = at::empty({x.size(0)}, x.options().dtype(at::kFloat));
   if (res) {
     vec = check_rows(*res, "residual", x) && vec;
@@ -93,7 +94,7 @@ std::vector<at::Tensor> rms_norm_fwd(at::Tensor x, MaybeTensor res, at::Tensor w
 
 // dw_acc: an fp32 slice that dw is added to; the second result is then empty
 std::vector<at::Tensor> rms_norm_bwd(at::Tensor dy, MaybeTensor dh, at::Tensor h, at::Tensor w,
-                                     at::Tensor rstd, MaybeTensor dw_acc) {
+                                     at::Tensor rstd, MaybeTensor dw_acc, at::IntArrayRef shape) {
   bool vec;
   RmsArgs a = norm_args(h, w, 0.0, vec);
   const c10::OptionalDeviceGuard guard(h.device());
@@ -108,7 +109,7 @@ std::vector<at::Tensor> rms_norm_bwd(at::Tensor dy, MaybeTensor dh, at::Tensor h
   if (dw_acc)
     TORCH_CHECK(dw_acc->device() == h.device() && dw_acc->scalar_type() == at::kFloat &&
                 dw_acc->is_contiguous() && dw_acc->numel() == a.H, "dw_acc must be an fp32 [hidden] slice");
-  auto dx = at::empty({h.size(0), h.size(1)}, h.options());
+  auto dx = at::empty(shape, h.options());
   auto dw = dw_acc ? at::Tensor() : at::empty({a.H}, w.options());
   if (a.R == 0) {
     if (dw.defined()) dw.zero_();
@@ -133,6 +134,11 @@ at::Tensor as_rows(const at::Tensor& t) {
 MaybeTensor as_rows(const MaybeTensor& t) { return t ? MaybeTensor(as_rows(*t)) : t; }
 MaybeTensor maybe(const at::Tensor& t) { return t.defined() ? MaybeTensor(t) : MaybeTensor(); }
 
+// gradients of gradients would be lost without a word
+void once() {
+  TORCH_CHECK(!at::GradMode::is_enabled(), "this operator has no second derivative: call it without create_graph");
+}
+
 // The autograd node lives here: in Python its forward and backward cost more
 // than the kernels on a small batch. `dw_acc`: an fp32 slice that the weight's
 // gradient is added to instead of being returned.
@@ -140,23 +146,24 @@ struct AddRmsNorm : public torch::autograd::Function<AddRmsNorm> {
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, at::Tensor x, MaybeTensor res,
                                                 at::Tensor w, double eps, MaybeTensor dw_acc) {
     w = w.contiguous();
-    auto r = rms_norm_fwd(as_rows(x), as_rows(res), w, eps);
+    auto r = rms_norm_fwd(as_rows(x), as_rows(res), w, eps, x.sizes());
     ctx->save_for_backward({r[1], w, r[2]});
     ctx->set_materialize_grads(false);
     ctx->saved_data["res"] = res.has_value();
     if (dw_acc) ctx->saved_data["acc"] = *dw_acc;
-    return {r[0].view(x.sizes()), res ? r[1].view(x.sizes()) : x};
+    return {r[0], res ? r[1] : x};
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                  torch::autograd::variable_list grads) {
+    once();
     const auto saved = ctx->get_saved_variables();
     const auto dy = grads[0], dh = grads[1];
     at::Tensor dx = dh, dw;
     if (dy.defined()) {  // y was used
       const auto acc = ctx->saved_data.find("acc");
-      auto r = rms_norm_bwd(as_rows(dy), as_rows(maybe(dh)), saved[0], saved[1], saved[2],
-                            acc == ctx->saved_data.end() ? MaybeTensor() : MaybeTensor(acc->second.toTensor()));
-      dx = r[0].view(dy.sizes());
+      auto r = rms_norm_bwd(as_rows(dy), as_rows(maybe(dh)), as_rows(saved[0]), saved[1], saved[2],
+                            acc == ctx->saved_data.end() ? MaybeTensor() : MaybeTensor(acc->second.toTensor()), dy.sizes());
+      dx = r[0];
       dw = r[1];
     }
     return {dx, ctx->saved_data["res"].toBool() ? dx : at::Tensor(), dw, at::Tensor(), at::Tensor()};
@@ -410,6 +417,7 @@ struct RelAttention : public torch::autograd::Function<RelAttention> {
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                  torch::autograd::variable_list grads) {
+    once();
     const auto s = ctx->get_saved_variables();
     auto r = rel_attn_bwd(aligned(grads[0]), s[0], s[4], s[5], ctx->saved_data["NH"].toInt(), ctx->saved_data["NKV"].toInt(),
                           s[1], s[2], maybe(s[3]), ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble());

@@ -127,6 +127,26 @@ def test_norm_empty_and_unused_outputs():
     assert torch.isfinite(w.grad).all()
 
 
+def test_norm_outputs_may_be_written_in_place():
+    x, r = (rand(2, 4, 64, dtype=torch.float32).requires_grad_() for _ in range(2))
+    w = rand(64, dtype=torch.float32).requires_grad_()
+    y, h = add_rms_norm(x, w, r)
+    y.mul_(2.0)
+    y.sum().backward()
+    assert torch.isfinite(x.grad).all()
+    y, h = add_rms_norm(x, w, r)
+    h.add_(1.0)  # the backward needs h as it was
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+def test_no_second_derivative():
+    x = rand(4, 64, dtype=torch.float32).requires_grad_()
+    y, _ = add_rms_norm(x, rand(64, dtype=torch.float32))
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(y.sum(), x, create_graph=True)
+
+
 def test_norm_not_finite_rows_stay_apart():
     x = rand(8, 512, dtype=torch.bfloat16)
     x[3, 5] = math.nan

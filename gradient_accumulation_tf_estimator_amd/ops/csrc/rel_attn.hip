@@ -388,13 +388,27 @@ __global__ __launch_bounds__(256, 2) void k_rel_fwd(RelArgs a, int tiles) {
     const int j0 = c * KC;
     if (bits != 0 && !(a.causal && j0 > i0 + 31)) {
       f16 s[2];
+      // where all 64 keys lie beyond the largest distance the bias goes into the
+      // exponent, and the products start from zero: 32 moves less
+      float flat = 0.f;
+      if (j0 + 63 - i0 <= -a.far || j0 - (i0 + 31) >= a.far) {
+        flat = (j0 < i0 ? low : high) * c2;
 #pragma unroll
-      for (int sub = 0; sub < 2; ++sub) s[sub] = bias_tile(bias, a.far, j0 + 32 * sub, i0, lane, low, high);
+        for (int sub = 0; sub < 2; ++sub) s[sub] = mfma(row_frag<D>(kt, 32 * sub + (lane & 31), 0, hi), q[0], (f16){});
 #pragma unroll
-      for (int t = 0; t < D / 16; ++t)
+        for (int t = 1; t < D / 16; ++t)
 #pragma unroll
-        for (int sub = 0; sub < 2; ++sub) s[sub] = mfma(row_frag<D>(kt, 32 * sub + (lane & 31), t, hi), q[t], s[sub]);
-      reads_ahead<D / 8>();
+          for (int sub = 0; sub < 2; ++sub) s[sub] = mfma(row_frag<D>(kt, 32 * sub + (lane & 31), t, hi), q[t], s[sub]);
+        reads_ahead<D / 8>();
+      } else {
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub) s[sub] = bias_tile(bias, a.far, j0 + 32 * sub, i0, lane, low, high);
+#pragma unroll
+        for (int t = 0; t < D / 16; ++t)
+#pragma unroll
+          for (int sub = 0; sub < 2; ++sub) s[sub] = mfma(row_frag<D>(kt, 32 * sub + (lane & 31), t, hi), q[t], s[sub]);
+        reads_ahead<D / 8>();
+      }
       if (bits != ~0ull || (a.causal && j0 + 63 > i0))
 #pragma unroll
         for (int sub = 0; sub < 2; ++sub)
@@ -402,7 +416,7 @@ __global__ __launch_bounds__(256, 2) void k_rel_fwd(RelArgs a, int tiles) {
       float top = larger(s[0][0], s[1][0]);
 #pragma unroll
       for (int r = 1; r < 16; ++r) top = larger(larger(top, s[0][r]), s[1][r]);
-      top *= c2;
+      top = fmaf(top, c2, flat);
       // the maximum moves only where it grew by more than 8 (a factor of 256,
       // far inside 32 bits and the same relative rounding in bf16): after the
       // first chunks the accumulators are hardly ever rescaled, and the two
@@ -417,13 +431,13 @@ __global__ __launch_bounds__(256, 2) void k_rel_fwd(RelArgs a, int tiles) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) o[dt][r] *= f;
       }
-      const float base = m == -INF ? 0.f : m;
+      const float base = flat - (m == -INF ? 0.f : m);
 #pragma unroll
       for (int sub = 0; sub < 2; ++sub) {
         float sum = 0.f;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          s[sub][r] = __builtin_amdgcn_exp2f(fmaf(s[sub][r], c2, -base));
+          s[sub][r] = __builtin_amdgcn_exp2f(fmaf(s[sub][r], c2, base));
           sum += s[sub][r];
         }
         l += sum;
@@ -474,7 +488,7 @@ __device__ __forceinline__ void diagonals_32(const f16& c, float* d, bool ib) {
 
 // ---------------- backward 1: dQ, D and the offsets' sums of dS ----------------
 template <int D>
-__global__ __launch_bounds__(256, 2) void k_rel_bwd_q(RelArgs a, int tiles) {
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_rel_bwd_q(RelArgs a, int tiles) {
   extern __shared__ __align__(16) char smem[];  // the tiles lie in the first 64 KB, which m0 reaches
   char* buf = smem;  // [2][K, V]
   constexpr int MAT = KC * 2 * D;
@@ -582,16 +596,25 @@ __global__ __launch_bounds__(256, 2) void k_rel_bwd_q(RelArgs a, int tiles) {
       if (on == 0 || (a.causal && j0 > i0 + 31)) continue;
       const char* ksub = kt + 64 * D * sub;
       const char* vsub = vt + 64 * D * sub;
-      f16 s = bias_tile(bias, a.far, j0, i0, lane, low, high);
-      f16 dp = {};
+      f16 s, dp = {};
+      const bool beyond = j0 + 31 - i0 <= -a.far || j0 - (i0 + 31) >= a.far;
+      float flat = 0.f;  // as in the forward
+      if (beyond) {
+        flat = (j0 < i0 ? low : high) * c2;
+        s = mfma(row_frag<D>(ksub, lane & 31, 0, hi), q[0], (f16){});
+      } else {
+        s = mfma(row_frag<D>(ksub, lane & 31, 0, hi), q[0], bias_tile(bias, a.far, j0, i0, lane, low, high));
+      }
+      dp = mfma(row_frag<D>(vsub, lane & 31, 0, hi), g[0], dp);
 #pragma unroll
-      for (int t = 0; t < D / 16; ++t) {
+      for (int t = 1; t < D / 16; ++t) {
         s = mfma(row_frag<D>(ksub, lane & 31, t, hi), q[t], s);
         dp = mfma(row_frag<D>(vsub, lane & 31, t, hi), g[t], dp);
       }
-      reads_ahead<D / 8>();
+      reads_ahead<D / 8 - 1>();
+      const float base = flat - lse;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c2, -lse));
+      for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c2, base));
       drop_rows(s, on, a.causal && j0 + 31 > i0, j0, i0, lane, 0.f);
       float whole = 0.f;
 #pragma unroll
@@ -602,7 +625,7 @@ __global__ __launch_bounds__(256, 2) void k_rel_bwd_q(RelArgs a, int tiles) {
       // sums of dS by offset: tiles beyond the largest distance in a register,
       // others along their diagonals
       rest += whole;
-      if (j0 + 31 - i0 <= -a.far || j0 - (i0 + 31) >= a.far) {
+      if (beyond) {
         float t = 0.f;
 #pragma unroll
         for (int r = 0; r < 16; ++r) t += s[r];

@@ -286,10 +286,9 @@ __device__ int mask_end(const unsigned char* mask, int end, int* lds) {
   return last;
 }
 
-// whether this lane's key of a chunk of 64 counts
-__device__ __forceinline__ bool key_on(const unsigned char* mask, int j0, int end) {
-  const int j = j0 + (threadIdx.x & 63);
-  return j < end && (!mask || mask[min(j, end - 1)]);
+// this lane's mask byte of a chunk of 64 keys
+__device__ __forceinline__ int key_byte(const unsigned char* mask, int j0, int end) {
+  return mask ? mask[min(j0 + (int)(threadIdx.x & 63), end - 1)] : 1;
 }
 
 // C rows whose key does not count, or lies behind the column's query -> fill
@@ -343,28 +342,28 @@ __global__ __launch_bounds__(256, 2) void k_rel_fwd(RelArgs a, int tiles) {
   const __bf16* v = k + a.NKV * D;
   const unsigned char* mask = a.mask ? a.mask + (long long)b * a.S : nullptr;
 
-  int end = a.causal ? min(a.S, tile * TILE + TILE) : a.S;
-  if (mask) end = mask_end(mask, end, ends);
-  const int chunks = (end + KC - 1) / KC;
+  int end = a.causal ? min(a.S, tile * TILE + TILE) : a.S;  // shorter once the mask is read
 
   Stage<D> st;
   st.init(a.width, a.width);
   unsigned long long bits = 0, next = 0;
-  bool key = false;
+  int key = 0;
   auto fetch = [&](int c) {
     char* to = buf + (c & 1) * 2 * MAT;
-    key = key_on(mask, c * KC, end);
+    key = key_byte(mask, c * KC, end);
     st.load(k, a.width, v, a.width, c * KC, end, to, to + MAT);
   };
   auto arrive = [&](int c) {
     char* to = buf + (c & 1) * 2 * MAT;
     st.wait();
-    next = __ballot(key);
+    next = __ballot(c * KC + lane < end && key != 0);
     st.clear(to, to + MAT, next);
   };
   // everything that the first chunk needs is on its way at once
-  if (chunks > 0) fetch(0);
+  fetch(0);
   const Bias first_bias(a, h);
+  if (mask) end = mask_end(mask, end, ends);
+  const int chunks = (end + KC - 1) / KC;
   b8 q[D / 16];
   const __bf16* qp = a.qkv + ((long long)b * a.S + min(i, a.S - 1)) * a.width + h * D;
 #pragma unroll
@@ -507,28 +506,28 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_rel_bwd_q(RelArgs a, i
   const __bf16* v = k + a.NKV * D;
   const unsigned char* mask = a.mask ? a.mask + (long long)b * a.S : nullptr;
 
-  int end = a.causal ? min(a.S, tile * TILE + TILE) : a.S;
-  if (mask) end = mask_end(mask, end, ends);
-  const int chunks = (end + KC - 1) / KC;
+  int end = a.causal ? min(a.S, tile * TILE + TILE) : a.S;  // shorter once the mask is read
 
   Stage<D> st;
   st.init(a.width, a.width);
   unsigned long long bits = 0, next = 0;
-  bool key = false;
+  int key = 0;
   auto fetch = [&](int c) {
     char* to = buf + (c & 1) * 2 * MAT;
-    key = key_on(mask, c * KC, end);
+    key = key_byte(mask, c * KC, end);
     st.load(k, a.width, v, a.width, c * KC, end, to, to + MAT);
   };
   auto arrive = [&](int c) {
     char* to = buf + (c & 1) * 2 * MAT;
     st.wait();
-    next = __ballot(key);
+    next = __ballot(c * KC + lane < end && key != 0);
     st.clear(to, to + MAT, next);
   };
   // everything that the first chunk needs is on its way at once
-  if (chunks > 0) fetch(0);
+  fetch(0);
   const Bias first_bias(a, h);
+  if (mask) end = mask_end(mask, end, ends);
+  const int chunks = (end + KC - 1) / KC;
   // a row past the end, or with nothing allowed, takes part as zeros
   const float lse = i < a.S ? a.lse[(long long)bh * a.S + i] : INF;
   const bool live = lse < INF || lse != lse;

@@ -64,7 +64,8 @@ struct RelArgs {
   int B, S, NH, NKV, D, width, buckets, far, causal, parts;
   float scale;
 };
-int rel_tiles(int S);
+#define GA_REL_TILE 128  // queries a workgroup
+__host__ __device__ inline int rel_tiles(int S) { return (S + GA_REL_TILE - 1) / GA_REL_TILE; }
 int rel_parts(int B, int S, int NH, int NKV);
 hipError_t rel_forward(const RelArgs& a, hipStream_t s);
 hipError_t rel_backward(const RelArgs& a, hipStream_t s);

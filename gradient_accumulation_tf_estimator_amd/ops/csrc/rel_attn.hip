@@ -46,7 +46,7 @@ typedef __attribute__((address_space(3))) char lds_char;
 #define INF __builtin_inff()
 
 constexpr int KC = 64;     // rows of a staged chunk
-constexpr int TILE = 128;  // rows of a workgroup: four waves of 32
+constexpr int TILE = GA_REL_TILE;  // rows of a workgroup: four waves of 32
 
 // ---- LDS tiles: [rows][D] bf16, 16-byte pieces XORed by a function of the row.
 // LDS serves 256 bytes at a time: sixteen neighbouring rows' pieces at one
@@ -252,8 +252,8 @@ __device__ __forceinline__ f16 bias_tile(const float* bias, int far, int row0, i
 // differ in work too: of some 64 workgroups at a time the longest start first.
 // `units` share nothing with each other, `per` columns of a unit share its keys
 // (query heads, or parts of them). Returns unit * per + column.
-__device__ __forceinline__ int place(int units, int per, int tiles, bool by_work, int& tile) {
-  int xcd = 0, step = 1, at = blockIdx.x, columns = units * per;
+__device__ __forceinline__ int place(int at, int units, int per, int tiles, bool by_work, int& tile) {
+  int xcd = 0, step = 1, columns = units * per;
   if ((units & 7) == 0) {
     xcd = at & 7;
     at >>= 3;
@@ -333,7 +333,7 @@ __global__ __launch_bounds__(256, 2) void k_rel_fwd(RelArgs a, int tiles) {
   int* ends = (int*)(bias + 4 * bias_len(a.far));
 
   int tile;
-  const int bh = place(a.B * a.NKV, a.NH / a.NKV, tiles, a.causal, tile);
+  const int bh = place(blockIdx.x, a.B * a.NKV, a.NH / a.NKV, tiles, a.causal, tile);
   const int h = bh % a.NH, b = bh / a.NH, hk = h / (a.NH / a.NKV);
   if (a.causal) tile = tiles - 1 - tile;  // the last tile has the most keys
   const int lane = threadIdx.x & 63, hi = lane >> 5;
@@ -497,7 +497,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_rel_bwd_q(RelArgs a, i
   float* sums = (float*)(ends + 4);  // [4 waves][2 halves][offs]
 
   int tile;
-  const int bh = place(a.B * a.NKV, a.NH / a.NKV, tiles, a.causal, tile);
+  const int bh = place(blockIdx.x, a.B * a.NKV, a.NH / a.NKV, tiles, a.causal, tile);
   const int h = bh % a.NH, b = bh / a.NH, hk = h / (a.NH / a.NKV);
   if (a.causal) tile = tiles - 1 - tile;  // the last tile has the most keys
   const int lane = threadIdx.x & 63, hi = lane >> 5, wave = threadIdx.x >> 6;
@@ -676,6 +676,48 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_rel_bwd_q(RelArgs a, i
   }
 }
 
+// dtable[n][h]: the offsets' sums over batches and tiles, then over the offsets
+// of a bucket; one workgroup a head, every sum in a fixed order. It needs the
+// dQ kernel alone, so it runs beside dK and dV, as their kernel's first NH
+// workgroups (as a kernel of its own behind them it took 4 to 14 us).
+template <int T>
+__device__ void sum_table(const RelArgs& a, int h, char* smem) {
+  constexpr int W = T / 64, COLS = 320;
+  float* part = (float*)smem;                                // [W][COLS]
+  float* sums = part + W * COLS;                             // [2 * far + 1]
+  short* map = (short*)(sums + 2 * GA_REL_MAX_DISTANCE + 1);  // [2 * far + 1]
+  const int offs = 2 * a.far + 1, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int n = a.B * rel_tiles(a.S);
+  const float* p = a.doff + (long long)h * n * offs;
+  for (int x = threadIdx.x; x < offs; x += T) map[x] = (short)min(max(a.map[x], 0), a.buckets - 1);
+  for (int x0 = 0; x0 < offs; x0 += COLS) {
+    float t[5] = {};
+#pragma unroll 4
+    for (int w = wave; w < n; w += W) {
+#pragma unroll
+      for (int i = 0; i < 5; ++i) t[i] += p[(long long)w * offs + min(x0 + 64 * i + lane, offs - 1)];
+    }
+#pragma unroll
+    for (int i = 0; i < 5; ++i) part[wave * COLS + 64 * i + lane] = t[i];
+    __syncthreads();
+    for (int x = threadIdx.x; x < COLS && x0 + x < offs; x += T) {
+      float s = 0.f;
+#pragma unroll
+      for (int i = 0; i < W; ++i) s += part[i * COLS + x];
+      sums[x0 + x] = s;
+    }
+    __syncthreads();
+  }
+  for (int bucket = wave; bucket < a.buckets; bucket += W) {
+    float t = 0.f;
+    for (int e = lane; e < offs; e += 64)
+      if (map[e] == bucket) t += sums[e];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) t += __shfl_xor(t, o, 64);
+    if (lane == 0) a.dtable[(long long)bucket * a.NH + h] = (__bf16)t;
+  }
+}
+
 // ---------------- backward 2: dK and dV; a wave owns 32 keys, chunks of 64 queries ----------------
 // Registers decide here: dK, dV, K and V of 32 keys are 256 of them at head size
 // 128. V is kept in LDS there, by eight waves that share a chunk instead of four:
@@ -695,8 +737,9 @@ __global__ __launch_bounds__(64 * kv_waves<D>(), D == 64 ? 3 : 2) void k_rel_bwd
   char* vt = (char*)(rows + 4 * KC);         // V_LDS: [KEYS][D]
   float* bias = (float*)(vt + (V_LDS ? KEYS * 2 * D : 0));
 
+  if ((int)blockIdx.x < a.NH) return sum_table<T>(a, blockIdx.x, smem);
   int tile;
-  const int column = place(a.B * a.NKV, a.parts, tiles, a.causal, tile);  // the first tile has the most queries
+  const int column = place(blockIdx.x - a.NH, a.B * a.NKV, a.parts, tiles, a.causal, tile);  // the first tile has the most queries
   const int part = column % a.parts, bk = column / a.parts;
   const int hk = bk % a.NKV, b = bk / a.NKV, group = a.NH / a.NKV;
   const int lane = threadIdx.x & 63, hi = lane >> 5;
@@ -843,45 +886,6 @@ __global__ __launch_bounds__(256) void k_rel_dkv(RelArgs a, long long n) {
   const long long b = row / a.S / a.NKV;
   const int head = c < a.D ? a.NH + hk : a.NH + a.NKV + hk;
   *(b4*)(a.dqkv + (b * a.S + s) * a.width + head * a.D + c % a.D) = v;
-}
-
-// dtable[n][h]: the offsets' sums over batches and tiles, then over the offsets
-// of a bucket; one workgroup a head, every sum in a fixed order. Latency bound:
-// a thread has up to twenty loads in flight.
-__global__ __launch_bounds__(1024) void k_rel_dtable(RelArgs a, int tiles) {
-  __shared__ float part[16][320];
-  __shared__ float sums[2 * GA_REL_MAX_DISTANCE + 1];
-  __shared__ short map[2 * GA_REL_MAX_DISTANCE + 1];
-  const int h = blockIdx.x, offs = 2 * a.far + 1, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  for (int x = threadIdx.x; x < offs; x += 1024) map[x] = (short)min(max(a.map[x], 0), a.buckets - 1);
-  const int n = a.B * tiles;
-  const float* p = a.doff + (long long)h * n * offs;
-  for (int x0 = 0; x0 < offs; x0 += 320) {
-    float t[5] = {};
-#pragma unroll 4
-    for (int w = wave; w < n; w += 16) {
-#pragma unroll
-      for (int i = 0; i < 5; ++i) t[i] += p[(long long)w * offs + min(x0 + 64 * i + lane, offs - 1)];
-    }
-#pragma unroll
-    for (int i = 0; i < 5; ++i) part[wave][64 * i + lane] = t[i];
-    __syncthreads();
-    if (threadIdx.x < 320 && x0 + threadIdx.x < offs) {
-      float s = 0.f;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s += part[i][threadIdx.x];
-      sums[x0 + threadIdx.x] = s;
-    }
-    __syncthreads();
-  }
-  for (int bucket = wave; bucket < a.buckets; bucket += 16) {
-    float t = 0.f;
-    for (int e = lane; e < offs; e += 64)
-      if (map[e] == bucket) t += sums[e];
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) t += __shfl_xor(t, o, 64);
-    if (lane == 0) a.dtable[(long long)bucket * a.NH + h] = (__bf16)t;
-  }
 }
 
 // ---------------- new tokens over a cache ----------------
@@ -1124,14 +1128,12 @@ hipError_t backward(const RelArgs& a, hipStream_t s) {
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL((k_rel_bwd_q<D>), dim3(a.B * a.NH * tiles), dim3(256), lds_q, s, a, tiles);
   if ((e = hipGetLastError()) != hipSuccess) return e;
-  hipLaunchKernelGGL((k_rel_bwd_kv<D>), dim3(a.B * a.NKV * a.parts * kv_tiles), dim3(T), lds_kv, s, a, kv_tiles);
+  hipLaunchKernelGGL((k_rel_bwd_kv<D>), dim3(a.NH + a.B * a.NKV * a.parts * kv_tiles), dim3(T), lds_kv, s, a, kv_tiles);
   if ((e = hipGetLastError()) != hipSuccess) return e;
   if (a.parts > 1) {
     const long long n = (long long)a.B * a.NKV * a.S * (D / 2);
     hipLaunchKernelGGL(k_rel_dkv, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, a, n);
-    if ((e = hipGetLastError()) != hipSuccess) return e;
   }
-  hipLaunchKernelGGL(k_rel_dtable, dim3(a.NH), dim3(1024), 0, s, a, tiles);
   return hipGetLastError();
 }
 
@@ -1149,8 +1151,6 @@ hipError_t token(const RelTokenArgs& a, hipStream_t s) {
 }
 
 }  // namespace
-
-int rel_tiles(int S) { return (S + TILE - 1) / TILE; }
 
 // Over how many workgroups the query heads that share a key/value head are
 // spread in the backward: one workgroup walks all queries of its heads, so

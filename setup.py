@@ -6,6 +6,8 @@ The .so lands at gradient_accumulation_tf_estimator_amd/ops/_ga_hip*.so so it
 travels with repo snapshots to GPU boxes (no JIT cache involved).
 """
 
+import glob
+import hashlib
 import os
 
 os.environ.setdefault("PYTORCH_ROCM_ARCH", "gfx950")
@@ -20,6 +22,14 @@ CSRC = os.path.join(HERE, "gradient_accumulation_tf_estimator_amd", "ops", "csrc
 # (v_pk_add/mul/fma_f32); they are kept out of every kernel. The host pass
 # does not know the feature and only warns.
 NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+
+# Objects are rebuilt when their command changes, not when a header does: the
+# headers' digest is part of the command.
+_digest = hashlib.sha256()
+for _h in sorted(glob.glob(os.path.join(CSRC, "*.h"))):
+    with open(_h, "rb") as _f:
+        _digest.update(_f.read())
+HEADERS = ["-DGA_HEADERS=0x" + _digest.hexdigest()[:8]]
 
 setup(
     name="gradient_accumulation_tf_estimator_amd",
@@ -58,7 +68,7 @@ setup(
             extra_compile_args={
                 "cxx": ["-O3"] + (["-fsanitize=address", "-g"]
                                   if os.environ.get("GA_ASAN") else []),
-                "nvcc": ["-O3", "--offload-arch=gfx950"] + NO_PACKED_FP32
+                "nvcc": ["-O3", "--offload-arch=gfx950"] + NO_PACKED_FP32 + HEADERS
                 + (["-fsanitize=address", "-g",
                     "-Xarch_device", "-fno-sanitize=all"]
                    if os.environ.get("GA_ASAN") else []),

@@ -8,7 +8,8 @@ which the reference calls on its list of gradients (optimization.py:84):
     norm = sqrt(sum_i sum(t_i^2));  out_i = t_i * clip_norm / max(norm, clip_norm)
 
 and where the norm is infinite or NaN every output is NaN. ``None`` entries are
-passed through. Sums are held in 64 bits. Nothing waits for the GPU: the norm
+passed through. Sums, and the norm that the outputs are clipped by, are held in
+64 bits; the results have no gradient. Nothing waits for the GPU: the norm
 stays on the device, and a call can be captured into a graph (which then holds
 the tensors' addresses).
 """
@@ -76,15 +77,33 @@ def clip_by_global_norm(tensors: Tensors, clip_norm: float, *,
     return dst, norm
 
 
+def _check_apart(got, dst):
+    """No output over another output, or over another tensor's input."""
+    def span(t):
+        size = 1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+        return t.data_ptr(), t.data_ptr() + size * t.element_size()
+
+    spans = sorted((*span(t), is_out) for d, t in zip(dst, got) if t.numel()
+                   for t, is_out in ((d, True), (t, False)) if is_out or t.data_ptr() != d.data_ptr())
+    out_end = any_end = 0
+    for lo, hi, is_out in spans:
+        if lo < (any_end if is_out else out_end):
+            raise RuntimeError("an output shares memory with another tensor of the list (is one listed twice?)")
+        any_end = max(any_end, hi)
+        out_end = max(out_end, hi) if is_out else out_end
+
+
 @torch.no_grad()
 def _plain_clip(got, dst, clip_norm):
     norm = _plain_norm(got)
     n = float(norm)
     coef = math.nan if not math.isfinite(n) else 1.0 if n <= clip_norm else clip_norm / n
     coef = torch.tensor(coef, dtype=torch.float32)
-    dst = dst or [torch.empty_like(t) for t in got]
     for d, t in zip(dst, got):
         if d.shape != t.shape or d.dtype != t.dtype or d.device != t.device:
             raise ValueError("an output must have its tensor's device, dtype and shape")
+    _check_apart(got, dst)
+    dst = dst or [torch.empty_like(t) for t in got]
+    for d, t in zip(dst, got):
         d.copy_(t.float() * coef)
     return norm.float(), dst

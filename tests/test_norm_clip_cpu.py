@@ -110,3 +110,24 @@ def test_clip_refusals():
     with pytest.raises(ValueError, match="output"):
         clip_by_global_norm([t], 1.0, out=[torch.ones(4)])
     assert float(global_norm([])) == 0 and clip_by_global_norm([None], 1.0)[0] == [None]
+
+
+def test_a_tensor_listed_twice_is_refused():
+    t, u = torch.ones(4), torch.ones(4)
+    with pytest.raises(RuntimeError, match="shares memory"):
+        clip_by_global_norm([t, t], 1.0, out=[t, t])
+    with pytest.raises(RuntimeError, match="shares memory"):
+        clip_by_global_norm([t, u], 1.0, out=[u, t])
+    big = torch.ones(8)
+    with pytest.raises(RuntimeError, match="shares memory"):
+        clip_by_global_norm([big[:5], big[3:]], 1.0, out=[big[:5], big[3:]])
+    assert (t == 1).all() and (u == 1).all() and (big == 1).all()
+    clip_by_global_norm([big[:4], big[4:]], 1.0, out=[big[:4], big[4:]])  # neighbours share nothing
+    assert abs(float(big.norm()) - 1.0) < 1e-6
+
+
+def test_fp8_scales_stay_in_the_normal_range():
+    x = torch.randn(3, 64)
+    for w in (1e-44, 1e-42, 1e-40):
+        q, s, _ = rms_norm_fp8(x, torch.full((64,), w))
+        assert torch.isfinite(q.float()).all() and (s >= torch.finfo(torch.float32).tiny).all()

@@ -3,8 +3,9 @@
 //   h = x + r            y = h * rstd * w,   rstd = 1 / sqrt(mean(h^2) + eps)
 //   dx = rstd * (w dy - n * mean(w dy n)) + dh,   n = h * rstd   (dr = dx)
 //   dw = sum over rows of dy n
-//   8-bit form: s = max|y| / 448 over a group of columns (1 where that is 0),
-//               q = e4m3(y / s)
+//   8-bit form: s = max|y| / 448 over a group of columns (1 where that is 0;
+//               at least 2^-126, or s itself would be rounded to a few bits or
+//               to zero), q = e4m3(y / s)
 //
 // Every form is bound by memory: one pass that keeps its row in registers,
 // 16-byte loads, one wave64 a row up to 1024 columns (statistics by lane
@@ -306,7 +307,7 @@ __global__ __launch_bounds__(256) void k_rms_fp8(RmsArgs a) {
         top = m[v];
         for (int o = lanes >> 1; o > 0; o >>= 1) top = Max::of(top, __shfl_xor(top, o, 64));
       }
-      const float scale = top == 0.f ? 1.f : top / 448.f;
+      const float part = top / 448.f, scale = top == 0.f ? 1.f : part < 0x1p-126f ? 0x1p-126f : part;
       if (lanes) {
         const int c = column<NT, MODE>(v, 0, t);
         if (c < a.H && (t % lanes) == 0) a.scales[row * scales + c / a.group] = scale;

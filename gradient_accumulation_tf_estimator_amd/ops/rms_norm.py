@@ -64,7 +64,8 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch
 def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None, *,
                  eps: float = 1e-6, group: int = 0) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """-> (q e4m3 [..., hidden], scales fp32 [..., groups], h). ``group`` columns
-    share a scale (0: the whole row, groups = 1); a group of zeros has scale 1.
+    share a scale (0: the whole row, groups = 1); a group of zeros has scale 1,
+    others at least 2^-126.
     For serving: nothing here has a gradient, so inputs that need one are
     refused while gradients are recorded."""
     _check(x, weight, residual)
@@ -82,8 +83,8 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch
     else:
         y, h = _plain(x, weight, residual, eps)
         y = y.reshape(x[..., 0].numel(), groups, x.shape[-1] // groups)
-        s = y.abs().amax(-1) / FP8_MAX
-        s = torch.where(s == 0, 1.0, s)
+        top = y.abs().amax(-1)
+        s = torch.where(top == 0, 1.0, (top / FP8_MAX).clamp_min(torch.finfo(top.dtype).tiny))
         q = (y / s[..., None]).to(torch.float8_e4m3fn)
     return q.view(x.shape), s.view(*x.shape[:-1], groups), x if residual is None else h.view(x.shape)
 

@@ -342,3 +342,41 @@ def test_clip_the_gradients_of_a_step():
     clip_by_global_norm([p.grad for p in params], 1.0, out=[p.grad for p in params])
     for p, w in zip(params, want):
         assert ((p.grad.double() - w).abs() <= 5 * U32 * w.abs() + 1e-30).all()
+
+
+@pytest.mark.parametrize("H,group", [(64, 0), (256, 32), (2048, 0), (4096, 128)])
+def test_norm_fp8_below_the_normal_range(H, group):
+    torch.manual_seed(17)
+    x = rand(5, H, dtype=torch.float32)
+    for w in (1e-44, 1e-42, 1e-40, 1e-37):
+        w = torch.full((H,), w, device="cuda")
+        q, s, _ = rms_norm_fp8(x, w, group=group)
+        _, _, y64 = reference(x, w, None, 1e-6)
+        per = s.double().repeat_interleave(group or H, 1)
+        assert (s >= torch.finfo(torch.float32).tiny).all()
+        # half a step of e4m3, and of a 32-bit value below the normal range
+        assert ((q.double() * per - y64).abs() <= (2.0**-4 + 60 * U32) * y64.abs() + 2.0**-10 * per + 2.0**-149).all()
+
+
+def test_norm_and_clip_in_inference_mode_on_a_stream():
+    torch.manual_seed(18)
+    norm = FusedAddRMSNorm(512).cuda().bfloat16()
+    x, r = rand(33, 512, dtype=torch.bfloat16), rand(33, 512, dtype=torch.bfloat16)
+
+    def both():
+        y, h = norm(x, r, return_sum=True)
+        q, s, _ = norm.forward_fp8(x, r, group=64)
+        out, n = clip_by_global_norm([y, h], 1.0)
+        return [y, h, q.view(torch.uint8), s, *out, n]
+
+    with torch.no_grad():
+        want = both()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side), torch.inference_mode():
+        got = both()
+        kept = got[0].clone()
+        clip_by_global_norm([kept], 0.5, out=[kept])
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert abs(float(kept.double().norm()) - 0.5) <= 0.5 * (half_step(torch.bfloat16) + U32)

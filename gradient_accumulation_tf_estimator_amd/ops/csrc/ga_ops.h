@@ -53,7 +53,8 @@ struct RelArgs {
   const int* map;             // [2 * far + 1], the bucket of each offset
   const unsigned char* mask;  // [B][S], 1 = attend, or null
   __bf16* out;                // [B][S][NH][D]
-  float* lse;                 // [B][NH][S], base 2; +inf for a row with nothing allowed
+  float* lse;                 // [2][B][NH][S]: base 2, +inf for a row with nothing allowed; a factor of P, 1 for
+                              // ordinary rows
   // backward
   const __bf16* dout;         // [B][S][NH][D]
   float* dsum;                // [B][NH][S]

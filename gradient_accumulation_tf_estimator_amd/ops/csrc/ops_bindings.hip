@@ -322,9 +322,9 @@ RelArgs rel_args(const at::Tensor& qkv, int64_t NH, int64_t NKV, const at::Tenso
   check_heads(NH, NKV, D);
   check_bias(table, map, qkv, NH);
   TORCH_CHECK(scale > 0 && std::isfinite(scale), "scale must be positive and finite");
-  // a chunk of 64 rows is addressed by 32 bits from its start
+  // a launch has fewer than 2^32 threads, 512 for each 128 rows of a head; a chunk of 64 rows is addressed by 32 bits from its start
   TORCH_CHECK(qkv.size(2) <= (1 << 23), "too many heads");
-  TORCH_CHECK(S < (1ll << 24) && B * NH * (S / 128 + 1) < (1ll << 31) && B * NKV * S * D < (1ll << 38), "too many rows");
+  TORCH_CHECK(S < (1ll << 24) && B * NH * (S / 128 + 1) < (1ll << 23), "too many rows");
   if (mask)
     TORCH_CHECK(mask->device() == qkv.device() && mask->scalar_type() == at::kByte && mask->is_contiguous() &&
                 mask->dim() == 2 && mask->size(0) == B && mask->size(1) == S, "mask must be a contiguous u8 [B, S] tensor");
@@ -346,13 +346,13 @@ RelArgs rel_args(const at::Tensor& qkv, int64_t NH, int64_t NKV, const at::Tenso
   return a;
 }
 
-// -> out [B, S, NH * D], lse [B, NH, S] (empty unless wanted)
+// -> out [B, S, NH * D], lse [2, B, NH, S] (empty unless wanted)
 std::vector<at::Tensor> rel_attn_fwd(at::Tensor qkv, int64_t NH, int64_t NKV, at::Tensor table, at::Tensor map,
                                      MaybeTensor mask, bool causal, double scale, bool want_lse) {
   RelArgs a = rel_args(qkv, NH, NKV, table, map, mask, causal, scale);
   const c10::OptionalDeviceGuard guard(qkv.device());
   auto out = at::empty({a.B, a.S, NH * a.D}, qkv.options());
-  auto lse = want_lse ? at::empty({a.B, NH, a.S}, qkv.options().dtype(at::kFloat)) : at::Tensor();
+  auto lse = want_lse ? at::empty({2, a.B, NH, a.S}, qkv.options().dtype(at::kFloat)) : at::Tensor();
   if (out.numel() == 0) return {out, lse};
   a.out = (__bf16*)out.data_ptr();
   a.lse = want_lse ? lse.data_ptr<float>() : nullptr;
@@ -371,14 +371,14 @@ std::vector<at::Tensor> rel_attn_bwd(at::Tensor dout, at::Tensor qkv, at::Tensor
                 t.numel() == (int64_t)a.B * a.S * NH * a.D && aligned16(t.data_ptr()),
                 "dout and out must be contiguous, 16-byte aligned bf16 [B, S, NH * D] tensors");
   TORCH_CHECK(lse.device() == qkv.device() && lse.scalar_type() == at::kFloat && lse.is_contiguous() &&
-              lse.numel() == (int64_t)a.B * NH * a.S, "lse must be the forward's");
+              lse.numel() == 2 * (int64_t)a.B * NH * a.S, "lse must be the forward's");
   auto dqkv = at::empty_like(qkv);
   auto dtable = at::empty_like(table);
   if (dqkv.numel() == 0) {
     dtable.zero_();
     return {dqkv, dtable};
   }
-  auto dsum = at::empty_like(lse);
+  auto dsum = at::empty({a.B, NH, a.S}, lse.options());
   auto doff = at::empty({(int64_t)a.B * NH * rel_tiles(a.S), 2 * a.far + 1}, lse.options());
   a.parts = rel_parts(a.B, a.S, a.NH, a.NKV);
   at::Tensor dkv;

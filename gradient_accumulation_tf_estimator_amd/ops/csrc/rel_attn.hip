@@ -46,6 +46,7 @@ typedef __attribute__((address_space(3))) char lds_char;
 #define INF __builtin_inff()
 
 constexpr int KC = 64;     // rows of a staged chunk
+constexpr float LARGE = 4096.f;  // of a row's maximum: from here on half its last bit is 2^-12, a relative 2^-12.5 of P
 constexpr int TILE = GA_REL_TILE;  // rows of a workgroup: four waves of 32
 
 // ---- LDS tiles: [rows][D] bf16, 16-byte pieces XORed by a function of the row.
@@ -161,6 +162,17 @@ struct Stage {
     __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0); the compiler knows it, and waits for no earlier load again
     asm volatile("" ::: "memory");
   }
+  __device__ __forceinline__ void scale(char* ty, const float* by, int r0, int end) {
+#pragma unroll 1
+    for (int i = 0; i < N; ++i) {
+      b8* p = (b8*)(ty + place(i));
+      const float f = by[min(r0 + row(i), end - 1)];
+      b8 v = *p;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = (__bf16)((float)v[e] * f);
+      *p = v;
+    }
+  }
   __device__ __forceinline__ void clear(char* tx, char* ty, unsigned long long on) {
     if (on != ~0ull) {
       const b8 zero = {};
@@ -179,13 +191,24 @@ struct Stage {
 __host__ __device__ __forceinline__ int bias_top(int far) { return (2 * far + 10) & ~3; }  // from here on all are the last offset's
 __host__ __device__ __forceinline__ int bias_len(int far) { return bias_top(far) + 4; }
 
-// A table value of the type's lowest stands for a mask, as -inf does: divided
-// by the scale it would leave 32 bits' range, and a sum of exponentials of it
-// would be lost in the saved logarithm.
+// Table values from -2^29 down (-1e9, the type's lowest) stand for a mask, as
+// -inf does: divided by the scale the lowest would leave 32 bits' range.
 __device__ __forceinline__ float as_bias(__bf16 t, float scale) {
   const float f = (float)t;
-  return f < -3.38e38f ? -INF : f / scale;
+  return f <= -536870912.f ? -INF : f / scale;
 }
+
+// a value that all lanes share, where a scalar register can hold it
+__device__ __forceinline__ float shared(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x)));
+}
+
+// A bias beyond the largest distance in the exponent, in base 2, and what that
+// product's rounding left out: with large values it would outweigh the scores.
+struct Flat {
+  float hi, lo;
+  __device__ __forceinline__ Flat(float bias, float c2) : hi(shared(bias * c2)), lo(shared(fabsf(hi) < INF ? fmaf(bias, c2, -hi) : 0.f)) {}
+};
 
 __device__ __forceinline__ void put_bias(float* bias, int len, int x, float v) {
 #pragma unroll
@@ -376,7 +399,8 @@ __global__ __launch_bounds__(256, 2) void k_rel_fwd(RelArgs a, int tiles) {
   f16 o[D / 32] = {};
   float m = -INF, l = 0.f;
   const float c2 = a.scale * LOG2E;
-  const float low = bias[0], high = bias[2 * a.far + 7];
+  const float low = shared(bias[0]), high = shared(bias[2 * a.far + 7]);
+  const Flat flat_low(low, c2), flat_high(high, c2);
 
   for (int c = 0; c < chunks; ++c) {
     bits = next;
@@ -389,9 +413,10 @@ __global__ __launch_bounds__(256, 2) void k_rel_fwd(RelArgs a, int tiles) {
       f16 s[2];
       // where all 64 keys lie beyond the largest distance the bias goes into the
       // exponent, and the products start from zero: 32 moves less
-      float flat = 0.f;
+      float flat = 0.f, flat_lo = 0.f;
       if (j0 + 63 - i0 <= -a.far || j0 - (i0 + 31) >= a.far) {
-        flat = (j0 < i0 ? low : high) * c2;
+        flat = j0 < i0 ? flat_low.hi : flat_high.hi;
+        flat_lo = j0 < i0 ? flat_low.lo : flat_high.lo;
 #pragma unroll
         for (int sub = 0; sub < 2; ++sub) s[sub] = mfma(row_frag<D>(kt, 32 * sub + (lane & 31), 0, hi), q[0], (f16){});
 #pragma unroll
@@ -430,7 +455,7 @@ __global__ __launch_bounds__(256, 2) void k_rel_fwd(RelArgs a, int tiles) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) o[dt][r] *= f;
       }
-      const float base = flat - (m == -INF ? 0.f : m);
+      const float base = flat - (m == -INF ? 0.f : m) + flat_lo;
 #pragma unroll
       for (int sub = 0; sub < 2; ++sub) {
         float sum = 0.f;
@@ -453,7 +478,14 @@ __global__ __launch_bounds__(256, 2) void k_rel_fwd(RelArgs a, int tiles) {
   l += __shfl_xor(l, 32, 64);
   if (i >= a.S) return;
   store_columns<D>(a.out + (((long long)b * a.S + i) * a.NH + h) * D, o, l == 0.f ? 0.f : 1.f / l, hi);
-  if (a.lse && hi == 0) a.lse[(long long)bh * a.S + i] = l == 0.f ? INF : m + __builtin_amdgcn_logf(l);
+  if (a.lse && hi == 0) {
+    // P = exp2(s - lse) * rest. A large maximum (a large bias that all keys of the
+    // row share) has no bits left for the sum's logarithm: the sum stays apart.
+    const bool apart = fabsf(m) >= LARGE && l != 0.f;
+    float* lse = a.lse + (long long)bh * a.S + i;
+    lse[0] = l == 0.f ? INF : apart ? m : m + __builtin_amdgcn_logf(l);
+    lse[(long long)a.B * a.NH * a.S] = apart ? 1.f / l : 1.f;
+  }
 }
 
 // lane i of each 16 takes lane i + N's value (N < 0: i - |N|), zero from outside
@@ -530,6 +562,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_rel_bwd_q(RelArgs a, i
   const int chunks = (end + KC - 1) / KC;
   // a row past the end, or with nothing allowed, takes part as zeros
   const float lse = i < a.S ? a.lse[(long long)bh * a.S + i] : INF;
+  const float rest_p = a.lse[(long long)a.B * a.NH * a.S + (long long)bh * a.S + min(i, a.S - 1)];  // 1, or 1 / sum
   const bool live = lse < INF || lse != lse;
   b8 q[D / 16], g[D / 16];
   float dsum = 0.f;
@@ -580,7 +613,9 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_rel_bwd_q(RelArgs a, i
   st.wait();
   if (chunks > 0) arrive(0);
   __syncthreads();
-  const float low = bias[0], high = bias[2 * a.far + 7];
+  const float low = shared(bias[0]), high = shared(bias[2 * a.far + 7]);
+  const Flat flat_low(low, c2), flat_high(high, c2);
+  dsum *= rest_p;
 
   for (int c = 0; c < chunks; ++c) {
     bits = next;
@@ -597,9 +632,10 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_rel_bwd_q(RelArgs a, i
       const char* vsub = vt + 64 * D * sub;
       f16 s, dp = {};
       const bool beyond = j0 + 31 - i0 <= -a.far || j0 - (i0 + 31) >= a.far;
-      float flat = 0.f;  // as in the forward
+      float flat = 0.f, flat_lo = 0.f;  // as in the forward
       if (beyond) {
-        flat = (j0 < i0 ? low : high) * c2;
+        flat = j0 < i0 ? flat_low.hi : flat_high.hi;
+        flat_lo = j0 < i0 ? flat_low.lo : flat_high.lo;
         s = mfma(row_frag<D>(ksub, lane & 31, 0, hi), q[0], (f16){});
       } else {
         s = mfma(row_frag<D>(ksub, lane & 31, 0, hi), q[0], bias_tile(bias, a.far, j0, i0, lane, low, high));
@@ -611,14 +647,14 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_rel_bwd_q(RelArgs a, i
         dp = mfma(row_frag<D>(vsub, lane & 31, t, hi), g[t], dp);
       }
       reads_ahead<D / 8 - 1>();
-      const float base = flat - lse;
+      const float base = flat - lse + flat_lo;
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c2, base));
       drop_rows(s, on, a.causal && j0 + 31 > i0, j0, i0, lane, 0.f);
       float whole = 0.f;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        dp[r] = s[r] * (dp[r] - dsum);
+        dp[r] = s[r] * fmaf(dp[r], rest_p, -dsum);
         whole += dp[r];
       }
       // sums of dS by offset: tiles beyond the largest distance in a register,
@@ -655,8 +691,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_rel_bwd_q(RelArgs a, i
     store_columns<D>(a.dqkv + ((long long)b * a.S + i) * a.width + h * D, dq, a.scale, hi);
   add(left_at - i0 + lane_off, left);
   rest += __shfl_xor(rest, 32, 64);
-  far_low += fmaf(-rest, mass_low, own_low);  // each half takes its own share
-  far_high += fmaf(-rest, mass_high, own_high);
+  far_low += fmaf(-rest, mass_low * rest_p, own_low);  // each half takes its own share
+  far_high += fmaf(-rest, mass_high * rest_p, own_high);
 #pragma unroll
   for (int x = 32; x > 0; x >>= 1) {
     far_low += __shfl_xor(far_low, x, 64);
@@ -722,7 +758,7 @@ __device__ void sum_table(const RelArgs& a, int h, char* smem) {
 // Registers decide here: dK, dV, K and V of 32 keys are 256 of them at head size
 // 128. V is kept in LDS there, by eight waves that share a chunk instead of four:
 // two waves a SIMD. Measured at 2x4093 causal, 16 heads over 4, D 128: 480 us
-// with V in registers, 325 us so; at 16x512, 12 heads, D 64: 45 us with V in
+// with V in registers, 345 us so; at 16x512, 12 heads, D 64: 45 us with V in
 // registers, 61 us in LDS with four waves, 85 us with eight.
 template <int D>
 constexpr int kv_waves() { return D == 64 ? 4 : 8; }
@@ -790,6 +826,12 @@ __global__ __launch_bounds__(64 * kv_waves<D>(), D == 64 ? 3 : 2) void k_rel_bwd
         st.wait();
         if (c * KC + lane >= a.S) row_lse = INF, row_d = 0.f;
         st.clear(to, to + MAT, __ballot(row_lse < INF || row_lse != row_lse));  // rows with nothing allowed too
+        if (__any(fabsf(row_lse) >= LARGE && row_lse < INF)) {
+          // the factor of P that stands apart goes into dO and D, rounding dO once more: dV takes P dO, dK takes P (dP - D)
+          const float* rest = lse + (long long)a.B * a.NH * a.S;
+          row_d *= rest[min(c * KC + lane, a.S - 1)];
+          st.scale(to + MAT, rest, c * KC, a.S);
+        }
         if (threadIdx.x < KC) {
           float* r = rows + (c & 1) * 2 * KC;
           r[threadIdx.x] = row_lse;
@@ -807,7 +849,7 @@ __global__ __launch_bounds__(64 * kv_waves<D>(), D == 64 ? 3 : 2) void k_rel_bwd
       }
       put(first);
       __syncthreads();
-      const float low = bias[0], high = bias[2 * a.far + 7];
+      const float low = shared(bias[0]), high = shared(bias[2 * a.far + 7]);
       for (int c = first; c < chunks; ++c) {
         if (c > first) __syncthreads();
         if (c + 1 < chunks) fetch(c + 1);

@@ -16,9 +16,11 @@ numbers outside the table are taken as the nearest one inside.
 * ``relative_attention_decode`` -- the serving form: a few new tokens of each
   sequence over its K/V cache.
 
-A table value of -inf, or of the type's lowest value, masks its offsets. What
-stands at a masked key or behind a sequence's end, NaN too, reaches no
-result. The kernels (ops/csrc/rel_attn.hip) take bf16; tensors on the CPU run
+A table value from -2^29 down (-1e9, the type's lowest value, -inf) masks its
+offsets; others are meant to be below 2^29. What stands at a key that the key
+mask drops or behind a sequence's end, NaN too, reaches no result. (Keys that
+only the causal order hides are ordinary data: a NaN in such a value row
+reaches the queries before it, as 0 * NaN.) The kernels (ops/csrc/rel_attn.hip) take bf16; tensors on the CPU run
 the same formulas in plain PyTorch.
 """
 
@@ -34,7 +36,7 @@ from . import require_hip
 
 MAX_DISTANCE = 512
 MAX_BUCKETS = 256
-_LOWEST = -3.38e38  # a table value from here down masks its offsets
+_LOWEST = -(2.0**29)  # a table value from here down masks its offsets
 
 
 def relative_position_buckets(num_buckets: int = 32, max_distance: int = 128,

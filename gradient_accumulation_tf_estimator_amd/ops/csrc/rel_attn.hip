@@ -933,11 +933,16 @@ __global__ __launch_bounds__(256) void k_rel_dkv(RelArgs a, long long n) {
 // ---------------- new tokens over a cache ----------------
 // The columns of a wave's tile are the rows (new token, head of the group) that
 // share a key/value head: one read of K and V serves them all. The keys are
-// split over `splits` workgroups and four waves each; a wave takes 32 keys at a
-// time, K straight into A fragments, V through its own LDS tile. The waves'
-// (maximum, sum, output) are joined in LDS, the workgroups' by k_rel_join.
+// split over `splits` workgroups and eight waves each (with four, 4x512 took 9.0 us
+// instead of 7.5); a wave takes 32 keys at a time, K straight into A fragments, V
+// through its own LDS tile. The waves' (maximum, sum, output) are joined in LDS,
+// the workgroups' by k_rel_join. Bound by the cache's bytes: 16 sequences of up to
+// 16384 tokens, 16 heads over 4, D 128: 90 us with the join, 4.5 TB/s of
+// the 4.9 that a copy reaches.
+constexpr int TOKEN_WAVES = 8;
 template <int D>
-__global__ __launch_bounds__(256) void k_rel_token(RelTokenArgs a, int row_tiles) {
+__global__ __launch_bounds__(512) void k_rel_token(RelTokenArgs a, int row_tiles) {
+  constexpr int W = TOKEN_WAVES, T = 64 * W;
   extern __shared__ __align__(16) char smem[];
   const int lane = threadIdx.x & 63, hi = lane >> 5, wave = threadIdx.x >> 6;
   const int group = a.NH / a.NKV, rows = group * a.Sq;
@@ -945,7 +950,7 @@ __global__ __launch_bounds__(256) void k_rel_token(RelTokenArgs a, int row_tiles
   const int rt = rest % row_tiles, hk = rest / row_tiles % a.NKV, b = rest / row_tiles / a.NKV;
   constexpr int MAT = 32 * 2 * D;
   char* vt = smem + wave * MAT;
-  int* map = (int*)(smem + 4 * MAT);             // [far + 1], offsets -far .. 0
+  int* map = (int*)(smem + W * MAT);             // [far + 1], offsets -far .. 0
   float* table = (float*)(map + a.far + 1);      // [buckets][heads of this tile]
   const int row = rt * 32 + (lane & 31);
   const int tok = min(row, rows - 1) / group, h = hk * group + min(row, rows - 1) % group;
@@ -954,7 +959,7 @@ __global__ __launch_bounds__(256) void k_rel_token(RelTokenArgs a, int row_tiles
   const int pos0 = len - a.Sq + rt * 32 / group;       // the first row's
 
   // keys in units of 32, spread evenly over the waves of all splits
-  const int units = (len + 31) / 32, waves = a.splits * 4, w = split * 4 + wave;
+  const int units = (len + 31) / 32, waves = a.splits * W, w = split * W + wave;
   const int u0 = (int)((long long)units * w / waves), u1 = (int)((long long)units * (w + 1) / waves);
   const __bf16* k = a.k + b * a.k_b + hk * a.k_h;
   const __bf16* v = a.v + b * a.v_b + hk * a.v_h;
@@ -977,8 +982,8 @@ __global__ __launch_bounds__(256) void k_rel_token(RelTokenArgs a, int row_tiles
   const __bf16* qp = a.q + b * a.q_b + tok * a.q_s + h * a.q_h;
 #pragma unroll
   for (int t = 0; t < D / 16; ++t) q[t] = *(const b8*)(qp + 16 * t + 8 * hi);
-  for (int x = threadIdx.x; x <= a.far; x += 256) map[x] = min(max(a.map[x], 0), a.buckets - 1);
-  for (int x = threadIdx.x; x < a.buckets * group; x += 256)
+  for (int x = threadIdx.x; x <= a.far; x += T) map[x] = min(max(a.map[x], 0), a.buckets - 1);
+  for (int x = threadIdx.x; x < a.buckets * group; x += T)
     table[x] = as_bias(a.table[(long long)(x / group) * a.NH + hk * group + x % group], a.scale);
   __syncthreads();
   const int mine = h - hk * group;
@@ -1050,10 +1055,11 @@ __global__ __launch_bounds__(256) void k_rel_token(RelTokenArgs a, int row_tiles
   }
   l += __shfl_xor(l, 32, 64);
 
-  // join the four waves: [4][32 rows][maximum, sum], then [32][D] by turns
+  // join the waves, eight rows at a time: [W][maximum, sum][32], the rows' own, [W][8][D + 4]
   __syncthreads();
-  float* stat = (float*)smem;          // [4][2][32]
-  float* acc = (float*)smem + 4 * 64;  // [32][D + 1]
+  float* stat = (float*)smem;
+  float* stats = stat + W * 64;
+  float* acc = stats + 64;
   if (hi == 0) {
     stat[wave * 64 + lane] = m;
     stat[wave * 64 + 32 + lane] = l;
@@ -1062,41 +1068,36 @@ __global__ __launch_bounds__(256) void k_rel_token(RelTokenArgs a, int row_tiles
   const int x = lane & 31;
   float top = -INF, sum = 0.f;
 #pragma unroll
-  for (int n = 0; n < 4; ++n) top = fmaxf(top, stat[n * 64 + x]);
+  for (int n = 0; n < W; ++n) top = fmaxf(top, stat[n * 64 + x]);
   const float base = top == -INF ? 0.f : top;
 #pragma unroll
-  for (int n = 0; n < 4; ++n) sum += stat[n * 64 + 32 + x] * __builtin_amdgcn_exp2f(stat[n * 64 + x] - base);
+  for (int n = 0; n < W; ++n) sum += stat[n * 64 + 32 + x] * __builtin_amdgcn_exp2f(stat[n * 64 + x] - base);
   const float f = __builtin_amdgcn_exp2f(m - base);
-  for (int n = 0; n < 4; ++n) {
-    if (wave == n)
-#pragma unroll
-      for (int dt = 0; dt < D / 32; ++dt)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          float* p = acc + x * (D + 1) + 32 * dt + crow(r, hi);
-          *p = n == 0 ? o[dt][r] * f : *p + o[dt][r] * f;
-        }
-    __syncthreads();
-  }
-  float* stats = (float*)smem;  // rows' maximum and sum, read by all below
   if (threadIdx.x < 32) {
     stats[threadIdx.x] = top;
     stats[32 + threadIdx.x] = sum;
   }
-  __syncthreads();
-  for (int e = threadIdx.x; e < 32 * D; e += 256) {
-    const int r = e / D, d = e % D, at = rt * 32 + r;
-    if (at >= rows) continue;
-    if (a.splits == 1) {
-      const float z = stats[32 + r];
-      a.out[(((long long)b * a.Sq + at / group) * a.NH + hk * group + at % group) * D + d] =
-          (__bf16)(z == 0.f ? 0.f : acc[r * (D + 1) + d] / z);
-    } else {
-      float* p = a.parts + (((long long)rest * a.splits + split) * 32 + r) * (D + 2);
-      p[d] = acc[r * (D + 1) + d];
-      if (d == 0) {
-        p[D] = stats[r];
-        p[D + 1] = stats[32 + r];
+  const int count = min(rows - rt * 32, 32);
+  for (int r0 = 0; r0 < count; r0 += 8) {
+    if (r0 > 0) __syncthreads();
+    if (x >= r0 && x < min(r0 + 8, count)) store_columns<D>(acc + (wave * 8 + x - r0) * (D + 4), o, f, hi);
+    __syncthreads();
+    for (int e = threadIdx.x; e < 8 * D; e += T) {
+      const int r = r0 + e / D, d = e % D, at = rt * 32 + r;
+      if (r >= count) break;
+      float t = 0.f;
+#pragma unroll
+      for (int n = 0; n < W; ++n) t += acc[(n * 8 + r - r0) * (D + 4) + d];
+      if (a.splits == 1) {
+        const float z = stats[32 + r];
+        a.out[(((long long)b * a.Sq + at / group) * a.NH + hk * group + at % group) * D + d] = (__bf16)(z == 0.f ? 0.f : t / z);
+      } else {
+        float* p = a.parts + (((long long)rest * a.splits + split) * 32 + r) * (D + 2);
+        p[d] = t;
+        if (d == 0) {
+          p[D] = stats[r];
+          p[D + 1] = stats[32 + r];
+        }
       }
     }
   }
@@ -1181,13 +1182,13 @@ hipError_t backward(const RelArgs& a, hipStream_t s) {
 
 template <int D>
 hipError_t token(const RelTokenArgs& a, hipStream_t s) {
+  constexpr int W = TOKEN_WAVES;
   const int group = a.NH / a.NKV, rows = group * a.Sq, row_tiles = (rows + 31) / 32;
-  size_t lds = 4 * 32 * 2 * D + 4 * (a.far + 1) + 4 * (size_t)a.buckets * group;
-  const size_t join = 4 * (4 * 64 + 32 * (D + 1));
-  if (lds < join) lds = join;
+  static_assert(4 * (W * 64 + 64 + W * 8 * (D + 4)) <= W * 32 * 2 * D, "the join fits where V was");
+  const size_t lds = W * 32 * 2 * D + 4 * (a.far + 1) + 4 * (size_t)a.buckets * group;
   const hipError_t e = allow(k_rel_token<D>, lds);
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL((k_rel_token<D>), dim3(a.B * a.NKV * row_tiles * a.splits), dim3(256), lds, s, a, row_tiles);
+  hipLaunchKernelGGL((k_rel_token<D>), dim3(a.B * a.NKV * row_tiles * a.splits), dim3(64 * W), lds, s, a, row_tiles);
   if (a.splits > 1) hipLaunchKernelGGL((k_rel_join<D>), dim3(a.B * a.NKV * rows), dim3(D), 0, s, a, row_tiles);
   return hipGetLastError();
 }
@@ -1206,12 +1207,18 @@ int rel_parts(int B, int S, int NH, int NKV) {
   return n;
 }
 
-// enough workgroups to fill the chip twice, but at least 128 keys a wave
+// Enough workgroups to fill the chip, but at least 64 keys a wave, since a second
+// kernel joins the parts: with 32, 4x512 (8 heads, D 64) takes 8.7 us instead of
+// 7.5, 4x1000 (8 heads over 2) 8.7 instead of 9.8; with 128, 1x16000 (8 over 1)
+// 12.4 instead of 10.9. Sequences differ in length, so workgroups of 4096 keys and
+// more are cut further: 16 sequences of 1 to 16384 tokens, 16 heads over 4, D 128:
+// 62 -> 54 us (8 over 8, D 64: 65 -> 52); 16x4096 would lose by it (18 -> 20).
 int rel_token_splits(int B, int Sq, int S, int NH, int NKV) {
   const long long rows = (long long)(NH / NKV) * Sq, base = (long long)B * NKV * ((rows + 31) / 32);
-  long long n = (512 + base - 1) / base;
+  long long n = (256 + base - 1) / base;
   const long long most = (S + 511) / 512;
   if (n > most) n = most;
+  while (n * 4096 <= S && base * n < 1024) n *= 2;
   return (int)(n < 1 ? 1 : n);
 }
 

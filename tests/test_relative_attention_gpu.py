@@ -520,3 +520,11 @@ def test_inference_mode_and_another_stream():
         got = both()
     side.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_token_long_caches_of_different_lengths():
+    torch.manual_seed(24)
+    m = relative_position_buckets(32, 128, False).cuda()
+    B, S, NH, NKV, D = 6, 9000, 4, 2, 64
+    lengths = torch.tensor([9000, 1, 4097, 0, 8191, 260], dtype=torch.int32, device="cuda")
+    check_token(rand(B, 2, NH, D), rand(B, S, NKV, D), rand(B, S, NKV, D), rand(32, NH), m, lengths)

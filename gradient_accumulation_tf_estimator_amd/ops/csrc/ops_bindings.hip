@@ -176,6 +176,8 @@ std::vector<at::Tensor> add_rms_norm(at::Tensor x, MaybeTensor res, at::Tensor w
 
 std::vector<at::Tensor> rms_norm_fp8(at::Tensor x, MaybeTensor res, at::Tensor w, double eps, int64_t group) {
   bool vec;
+  auto shape = x.sizes().vec();  // the outputs have the caller's shape
+  const auto given = x;
   x = as_rows(x);
   res = as_rows(res);
   w = w.contiguous();
@@ -184,9 +186,10 @@ std::vector<at::Tensor> rms_norm_fp8(at::Tensor x, MaybeTensor res, at::Tensor w
   TORCH_CHECK(group == 0 || group == 32 || group == 64 || group == 128, "group must be 0 (a row), 32, 64 or 128");
   TORCH_CHECK(group == 0 || a.H % group == 0, "hidden must be a multiple of the group");
   const int64_t groups = group ? a.H / group : 1;
-  auto q = at::empty({x.size(0), x.size(1)}, x.options().dtype(at::kFloat8_e4m3fn));
-  auto scales = at::empty({x.size(0), groups}, x.options().dtype(at::kFloat));
-  auto h = res ? at::empty({x.size(0), x.size(1)}, x.options()) : x;
+  auto q = at::empty(shape, x.options().dtype(at::kFloat8_e4m3fn));
+  auto h = res ? at::empty(shape, x.options()) : given;
+  shape.back() = groups;
+  auto scales = at::empty(shape, x.options().dtype(at::kFloat));
   if (res) {
     vec = check_rows(*res, "residual", x) && vec;
     a.res = res->data_ptr();

@@ -77,16 +77,15 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch
         raise ValueError(f"hidden {x.shape[-1]} is no multiple of group {group}")
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
         raise RuntimeError("rms_norm_fp8 has no gradient: call it under torch.no_grad()")
-    groups = x.shape[-1] // group if group else 1
     if x.is_cuda:
-        q, s, h = require_hip().rms_norm_fp8(x, residual, weight, eps, group)
-    else:
-        y, h = _plain(x, weight, residual, eps)
-        y = y.reshape(x[..., 0].numel(), groups, x.shape[-1] // groups)
-        top = y.abs().amax(-1)
-        s = torch.where(top == 0, 1.0, (top / FP8_MAX).clamp_min(torch.finfo(top.dtype).tiny))
-        q = (y / s[..., None]).to(torch.float8_e4m3fn)
-    return q.view(x.shape), s.view(*x.shape[:-1], groups), x if residual is None else h.view(x.shape)
+        return tuple(require_hip().rms_norm_fp8(x, residual, weight, eps, group))
+    groups = x.shape[-1] // group if group else 1
+    y, h = _plain(x, weight, residual, eps)
+    y = y.reshape(*x.shape[:-1], groups, x.shape[-1] // groups)
+    top = y.abs().amax(-1)
+    s = torch.where(top == 0, 1.0, (top / FP8_MAX).clamp_min(torch.finfo(top.dtype).tiny))
+    q = (y / s[..., None]).to(torch.float8_e4m3fn)
+    return q.view(x.shape), s, h
 
 
 class FusedAddRMSNorm(nn.Module):

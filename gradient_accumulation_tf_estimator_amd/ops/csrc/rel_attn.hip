@@ -227,9 +227,10 @@ __device__ __forceinline__ void put_bias(float* bias, int len, int x, float v) {
 }
 
 // In two steps, so that the two dependent loads of an entry run beside the
-// kernel's other first loads: the constructor issues them, `put` stores.
+// kernel's other first loads: the constructor issues them, `put` stores. T threads;
+// mirrored: the offset of an entry with its sign turned.
+template <int T = 256, bool MIRRORED = false>
 struct Bias {
-  static constexpr int T = 256;
   static constexpr int N = (2 * GA_REL_MAX_DISTANCE + 17 + T - 1) / T;
   __bf16 t[N];
   int len;
@@ -239,7 +240,7 @@ struct Bias {
     for (int i = 0; i < N; ++i) {
       if (i * T >= len + 3) break;
       const int d = min(max((int)threadIdx.x + T * i - 7 - a.far, -a.far), a.far);
-      n[i] = a.map[d + a.far];
+      n[i] = a.map[(MIRRORED ? -d : d) + a.far];
     }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -342,18 +343,44 @@ __device__ __forceinline__ void drop_rows(f16& c, unsigned bits, bool diag, int 
   }
 }
 
-template <int D, typename E>
-__device__ __forceinline__ void store_columns(E* row, const f16* c, float mul, int hi) {
-  typedef __attribute__((ext_vector_type(4))) E e4;
+template <int D>
+__device__ __forceinline__ void store_columns(float* row, const f16* c, float mul, int hi) {
 #pragma unroll
   for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      e4 v;
+      f4 v;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = (E)(c[dt][4 * g + e] * mul);
-      *(e4*)(row + 32 * dt + 8 * g + 4 * hi) = v;
+      for (int e = 0; e < 4; ++e) v[e] = c[dt][4 * g + e] * mul;
+      *(f4*)(row + 32 * dt + 8 * g + 4 * hi) = v;
     }
+}
+
+// The wave's 32 columns of C as bf16 rows of memory, `count` of them, by way of its
+// own 64 D bytes of LDS: whole rows, 16 bytes a lane. From the registers every store
+// would touch 32 rows with 16 bytes each, four to eight times the requests.
+template <int D>
+__device__ __forceinline__ void store_rows(char* tile, __bf16* to, long long stride, int count, const f16* c, float mul, int lane) {
+  const int hi = lane >> 5;
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      b4 v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = (__bf16)(c[dt][4 * g + e] * mul);
+      *(b4*)(tile + piece<D>(lane & 31, 4 * dt + g) + 8 * hi) = v;
+    }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll
+  for (int n = 0; n < D / 16; ++n) {
+    const int r = (lane + 64 * n) / (D / 8), p = lane % (D / 8);
+    const b8 v = *(const b8*)(tile + piece<D>(r, p));
+    if (r < count) *(b8*)(to + r * stride + 8 * p) = v;
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
 }
 
 // ---------------- forward: a wave owns 32 queries, chunks of 64 keys ----------------
@@ -395,7 +422,7 @@ __global__ __launch_bounds__(256, 2) void k_rel_fwd(RelArgs a, int tiles) {
   };
   // everything that the first chunk needs is on its way at once
   fetch(0);
-  const Bias first_bias(a, h);
+  const Bias<> first_bias(a, h);
   if (mask) end = mask_end(mask, end, ends);
   const int chunks = (end + KC - 1) / KC;
   b8 q[D / 16];
@@ -487,9 +514,10 @@ __global__ __launch_bounds__(256, 2) void k_rel_fwd(RelArgs a, int tiles) {
     if (c + 1 < chunks) arrive(c + 1);
   }
   l += __shfl_xor(l, 32, 64);
-  if (i >= a.S) return;
-  store_columns<D>(a.out + (((long long)b * a.S + i) * a.NH + h) * D, o, l == 0.f ? 0.f : 1.f / l, hi);
-  if (a.lse && hi == 0) {
+  __syncthreads();  // the tiles are read
+  store_rows<D>(smem + (threadIdx.x >> 6) * 64 * D, a.out + (((long long)b * a.S + i0) * a.NH + h) * D, a.NH * D, a.S - i0, o,
+                l == 0.f ? 0.f : 1.f / l, lane);
+  if (i < a.S && a.lse && hi == 0) {
     // P = exp2(s - lse) * rest. A large maximum (a large bias that all keys of the
     // row share) has no bits left for the sum's logarithm: the sum stays apart.
     const bool apart = fabsf(m) >= LARGE && l != 0.f;
@@ -569,7 +597,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_rel_bwd_q(RelArgs a, i
   };
   // everything that the first chunk needs is on its way at once
   fetch(0);
-  const Bias first_bias(a, h);
+  const Bias<> first_bias(a, h);
   if (mask) end = mask_end(mask, end, ends);
   const int chunks = (end + KC - 1) / KC;
   // a row past the end, or with nothing allowed, takes part as zeros
@@ -699,8 +727,6 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_rel_bwd_q(RelArgs a, i
     }
     if (c + 1 < chunks) arrive(c + 1);
   }
-  if (i < a.S)
-    store_columns<D>(a.dqkv + ((long long)b * a.S + i) * a.width + h * D, dq, a.scale, hi);
   add(left_at - i0 + lane_off, left);
   rest += __shfl_xor(rest, 32, 64);
   far_low += fmaf(-rest, mass_low * rest_p, own_low);  // each half takes its own share
@@ -715,6 +741,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_rel_bwd_q(RelArgs a, i
     mine[offs - 1] += far_high;
   }
   __syncthreads();
+  store_rows<D>(smem + wave * 64 * D, a.dqkv + ((long long)b * a.S + i0) * a.width + h * D, a.width, a.S - i0, dq, a.scale, lane);
   float* to = a.doff + (((long long)h * a.B + b) * tiles + tile) * offs;
   for (int x = threadIdx.x; x < offs; x += 256) {
     float t = 0.f;
@@ -782,13 +809,13 @@ __global__ __launch_bounds__(64 * kv_waves<D>(), D == 64 ? 3 : 2) void k_rel_bwd
   extern __shared__ __align__(16) char smem[];  // the chunks lie in the first 64 KB, which m0 reaches
   char* buf = smem;                             // [2][Q, dO]
   constexpr int MAT = KC * 2 * D;
-  float* rows = (float*)(smem + 4 * MAT);    // [2][lse, D][64]
+  float* rows = (float*)(smem + 4 * MAT);    // [2][lse, -D][64]
   char* vt = (char*)(rows + 4 * KC);         // V_LDS: [KEYS][D]
   float* bias = (float*)(vt + (V_LDS ? KEYS * 2 * D : 0));
 
   if ((int)blockIdx.x < a.NH) return sum_table<T>(a, blockIdx.x, smem);
   int tile;
-  const int column = place(blockIdx.x - a.NH, a.B * a.NKV, a.parts, tiles, a.causal, tile);  // the first tile has the most queries
+  const int column = place(blockIdx.x - a.NH, a.B * a.NKV, a.parts, tiles, a.causal || a.mask, tile);  // the first tile has the most queries, and keys that count
   const int part = column % a.parts, bk = column / a.parts;
   const int hk = bk % a.NKV, b = bk / a.NKV, group = a.NH / a.NKV;
   const int lane = threadIdx.x & 63, hi = lane >> 5;
@@ -796,6 +823,47 @@ __global__ __launch_bounds__(64 * kv_waves<D>(), D == 64 ? 3 : 2) void k_rel_bwd
   const int j0 = tile * KEYS + (threadIdx.x >> 6) * 32, j = j0 + (lane & 31);
   const bool keep = j < a.S && (!a.mask || a.mask[(long long)b * a.S + min(j, a.S - 1)]);
   const bool work = __any(keep);  // this wave has a key that counts
+
+  const int first = a.causal ? tile * KEYS / KC : 0, chunks = (a.S + KC - 1) / KC;
+  Stage<D, T> st;
+  st.init(a.width, a.NH * D);
+  float row_lse = 0.f, row_d = 0.f;
+  const __bf16 *q, *g;
+  const float *lse, *dsum;
+  auto fetch = [&](int c) {
+    char* to = buf + (c & 1) * 2 * MAT;
+    const int r = c * KC + lane;
+    row_lse = lse[min(r, a.S - 1)];
+    row_d = dsum[min(r, a.S - 1)];
+    st.load(q, a.width, g, a.NH * D, c * KC, a.S, to, to + MAT);
+  };
+  auto put = [&](int c) {
+    char* to = buf + (c & 1) * 2 * MAT;
+    st.wait();
+    if (c * KC + lane >= a.S) row_lse = INF, row_d = 0.f;
+    st.clear(to, to + MAT, __ballot(row_lse < INF || row_lse != row_lse));  // rows with nothing allowed too
+    if (__any(fabsf(row_lse) >= LARGE && row_lse < INF)) {
+      // the factor of P that stands apart goes into dO and D, rounding dO once more: dV takes P dO, dK takes P (dP - D)
+      const float* rest = lse + (long long)a.B * a.NH * a.S;
+      row_d *= rest[min(c * KC + lane, a.S - 1)];
+      st.scale(to + MAT, rest, c * KC, a.S);
+    }
+    if (threadIdx.x < KC) {
+      float* r = rows + (c & 1) * 2 * KC;
+      r[threadIdx.x] = row_lse;
+      r[KC + threadIdx.x] = -row_d;
+    }
+  };
+  auto begin = [&](int n) {  // the first chunk and the bias of the n-th query head are on their way
+    const int h = hk * group + n;
+    q = a.qkv + (long long)b * a.S * a.width + h * D;
+    g = a.dout + ((long long)b * a.S * a.NH + h) * D;
+    lse = a.lse + (long long)(b * a.NH + h) * a.S;
+    dsum = a.dsum + (long long)(b * a.NH + h) * a.S;
+    fetch(first);
+    return Bias<T, true>(a, h);
+  };
+  auto next = begin(part);
 
   b8 k[D / 16], v[V_LDS ? 1 : D / 16];
   {
@@ -814,52 +882,15 @@ __global__ __launch_bounds__(64 * kv_waves<D>(), D == 64 ? 3 : 2) void k_rel_bwd
   }
   f16 dk[D / 32] = {}, dv[D / 32] = {};
   const float c2 = a.scale * LOG2E;
-  const int first = a.causal ? tile * KEYS / KC : 0, chunks = (a.S + KC - 1) / KC;
-  Stage<D, T> st;
-  st.init(a.width, a.NH * D);
-  float row_lse = 0.f, row_d = 0.f;
   st.wait();
 
   if (__syncthreads_or(work))
     for (int n = part; n < group; n += a.parts) {
-      const int h = hk * group + n, bh = b * a.NH + h;
-      const __bf16* q = a.qkv + (long long)b * a.S * a.width + h * D;
-      const __bf16* g = a.dout + ((long long)b * a.S * a.NH + h) * D;
-      const float* lse = a.lse + (long long)bh * a.S;
-      const float* dsum = a.dsum + (long long)bh * a.S;
-      auto fetch = [&](int c) {
-        char* to = buf + (c & 1) * 2 * MAT;
-        const int r = c * KC + lane;
-        row_lse = lse[min(r, a.S - 1)];
-        row_d = dsum[min(r, a.S - 1)];
-        st.load(q, a.width, g, a.NH * D, c * KC, a.S, to, to + MAT);
-      };
-      auto put = [&](int c) {
-        char* to = buf + (c & 1) * 2 * MAT;
-        st.wait();
-        if (c * KC + lane >= a.S) row_lse = INF, row_d = 0.f;
-        st.clear(to, to + MAT, __ballot(row_lse < INF || row_lse != row_lse));  // rows with nothing allowed too
-        if (__any(fabsf(row_lse) >= LARGE && row_lse < INF)) {
-          // the factor of P that stands apart goes into dO and D, rounding dO once more: dV takes P dO, dK takes P (dP - D)
-          const float* rest = lse + (long long)a.B * a.NH * a.S;
-          row_d *= rest[min(c * KC + lane, a.S - 1)];
-          st.scale(to + MAT, rest, c * KC, a.S);
-        }
-        if (threadIdx.x < KC) {
-          float* r = rows + (c & 1) * 2 * KC;
-          r[threadIdx.x] = row_lse;
-          r[KC + threadIdx.x] = row_d;
-        }
-      };
-      __syncthreads();  // the last head's tiles are read
-      fetch(first);
-      // (in a plain loop: this kernel has no register to spare)
-#pragma unroll 1
-      for (int x = threadIdx.x; x < bias_len(a.far) + 3; x += T) {
-        const int d = min(max(a.far + 7 - x, -a.far), a.far);  // mirrored
-        const int at = min(max(a.map[d + a.far], 0), a.buckets - 1);
-        put_bias(bias, bias_len(a.far), x, as_bias(a.table[(long long)at * a.NH + h], a.scale));
+      if (n != part) {
+        __syncthreads();  // the last head's tiles are read
+        next = begin(n);
       }
+      next.put(a.scale, bias);
       put(first);
       __syncthreads();
       const float low = shared(bias[0]), high = shared(bias[2 * a.far + 7]);
@@ -876,7 +907,13 @@ __global__ __launch_bounds__(64 * kv_waves<D>(), D == 64 ? 3 : 2) void k_rel_bwd
           const char* qs = qt + 64 * D * sub;
           const char* gs = gt + 64 * D * sub;
           // rows are queries here: the mirrored bias of row - column
-          f16 s = bias_tile(bias, a.far, i0, j0, lane, low, high), dp = {};
+          f16 s = bias_tile(bias, a.far, i0, j0, lane, low, high), dp;  // dP starts from -D: no subtraction later
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const f4 d = *(const f4*)(rl + KC + 32 * sub + 8 * x + 4 * hi);
+#pragma unroll
+            for (int y = 0; y < 4; ++y) dp[4 * x + y] = d[y];
+          }
 #pragma unroll
           for (int t = 0; t < D / 16; ++t) {
             s = mfma(row_frag<D>(qs, lane & 31, t, hi), k[t], s);
@@ -896,11 +933,7 @@ __global__ __launch_bounds__(64 * kv_waves<D>(), D == 64 ? 3 : 2) void k_rel_bwd
             for (int y = 0; y < 4; ++y) s[4 * x + y] = __builtin_amdgcn_exp2f(fmaf(s[4 * x + y], c2, -e[y]));
           }
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const f4 d = *(const f4*)(rl + KC + 32 * sub + 8 * x + 4 * hi);
-#pragma unroll
-            for (int y = 0; y < 4; ++y) dp[4 * x + y] = (dp[4 * x + y] - d[y]) * s[4 * x + y];
-          }
+          for (int r = 0; r < 16; ++r) dp[r] *= s[r];
 #pragma unroll
           for (int ks = 0; ks < 2; ++ks) {
             const b8 p = pack(s, ks), ds = pack(dp, ks);
@@ -914,15 +947,22 @@ __global__ __launch_bounds__(64 * kv_waves<D>(), D == 64 ? 3 : 2) void k_rel_bwd
         if (c + 1 < chunks) put(c + 1);
       }
     }
-  if (j >= a.S) return;
   // a masked key's column holds what its zeroed K and V gave: it has no gradient
-  const f16 none[D / 32] = {};
-  auto write = [&](auto* at, int step) {
-    store_columns<D>(at, keep ? dk : none, a.scale, hi);
-    store_columns<D>(at + step, keep ? dv : none, 1.f, hi);
-  };
-  if (a.parts > 1) write(a.dkv + (((long long)part * a.B * a.NKV + bk) * a.S + j) * 2 * D, D);
-  else write(a.dqkv + ((long long)b * a.S + j) * a.width + (a.NH + hk) * D, a.NKV * D);
+  if (!keep)
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt) dk[dt] = dv[dt] = (f16){};
+  if (a.parts > 1) {
+    if (j >= a.S) return;
+    float* to = a.dkv + (((long long)part * a.B * a.NKV + bk) * a.S + j) * 2 * D;
+    store_columns<D>(to, dk, a.scale, hi);
+    store_columns<D>(to + D, dv, 1.f, hi);
+  } else {
+    __syncthreads();  // the chunks are read
+    char* own = smem + (threadIdx.x >> 6) * 64 * D;
+    __bf16* to = a.dqkv + ((long long)b * a.S + j0) * a.width + (a.NH + hk) * D;
+    store_rows<D>(own, to, a.width, a.S - j0, dk, a.scale, lane);
+    store_rows<D>(own, to + a.NKV * D, a.width, a.S - j0, dv, 1.f, lane);
+  }
 }
 
 // the parts' dK and dV, added in order: four columns a thread; long 24 us (151 MB)

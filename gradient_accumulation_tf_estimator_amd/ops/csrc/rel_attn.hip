@@ -283,7 +283,7 @@ __device__ __forceinline__ f16 bias_tile(const float* bias, int far, int row0, i
 // by turns, and each XCD has an L2 of its own, so all tiles of the heads that
 // share keys go to one XCD; neighbouring units (a batch's key heads) go to
 // different ones, since batches differ in length. Under the causal mask tiles
-// differ in work too: of some 64 workgroups at a time the longest start first.
+// differ in work too (and key tiles of a padded batch do): of some 64 workgroups at a time the longest start first.
 // `units` share nothing with each other, `per` columns of a unit share its keys
 // (query heads, or parts of them). Returns unit * per + column.
 __device__ __forceinline__ int place(int at, int units, int per, int tiles, bool by_work, int& tile) {
@@ -358,7 +358,8 @@ __device__ __forceinline__ void store_columns(float* row, const f16* c, float mu
 
 // The wave's 32 columns of C as bf16 rows of memory, `count` of them, by way of its
 // own 64 D bytes of LDS: whole rows, 16 bytes a lane. From the registers every store
-// would touch 32 rows with 16 bytes each, four to eight times the requests.
+// would touch 32 rows with 16 bytes each: dK and dV took 54 us instead of 47.5 at
+// 16x512 padded, 8 heads, D 128. The fp32 parts gained nothing by it.
 template <int D>
 __device__ __forceinline__ void store_rows(char* tile, __bf16* to, long long stride, int count, const f16* c, float mul, int lane) {
   const int hi = lane >> 5;
@@ -384,7 +385,7 @@ __device__ __forceinline__ void store_rows(char* tile, __bf16* to, long long str
 }
 
 // ---------------- forward: a wave owns 32 queries, chunks of 64 keys ----------------
-// padded 24 us (matrix unit 21 % busy), long 173 us (46 %, 790 TFLOP/s)
+// padded 24 us (matrix unit 22 % busy), long 163 us (46 %, 841 TFLOP/s)
 template <int D>
 __global__ __launch_bounds__(256, 2) void k_rel_fwd(RelArgs a, int tiles) {
   extern __shared__ __align__(16) char smem[];  // the tiles lie in the first 64 KB, which m0 reaches
@@ -557,7 +558,7 @@ __device__ __forceinline__ void diagonals_32(const f16& c, float* d, bool ib) {
 }
 
 // ---------------- backward 1: dQ, D and the offsets' sums of dS ----------------
-// padded 37 us (matrix unit 19 % busy), long 265 us (43 %, 776 TFLOP/s)
+// padded 38 us (matrix unit 19 % busy), long 243 us (42 %, 848 TFLOP/s)
 template <int D>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_rel_bwd_q(RelArgs a, int tiles) {
   extern __shared__ __align__(16) char smem[];  // the tiles lie in the first 64 KB, which m0 reaches
@@ -796,10 +797,10 @@ __device__ void sum_table(const RelArgs& a, int h, char* smem) {
 // ---------------- backward 2: dK and dV; a wave owns 32 keys, chunks of 64 queries ----------------
 // Registers decide here: dK, dV, K and V of 32 keys are 256 of them at head size
 // 128. V is kept in LDS there, by eight waves that share a chunk instead of four:
-// two waves a SIMD. padded 48 us (matrix unit 20 % busy), long 350 us (41 %, 784
-// TFLOP/s), the table's sums among them. Measured at 2x4093 causal, 16 heads over 4, D 128: 480 us
-// with V in registers, 345 us so; at 16x512, 12 heads, D 64: 45 us with V in
-// registers, 61 us in LDS with four waves, 85 us with eight.
+// two waves a SIMD (long: 480 us with V in registers, 340 so, when that step was
+// taken; padded: 45 us with V in registers, 61 in LDS with four waves, 85 with
+// eight). padded 44 us (matrix unit 21 % busy), long 297 us (43 %, 925 TFLOP/s),
+// the table's sums among them.
 template <int D>
 constexpr int kv_waves() { return D == 64 ? 4 : 8; }
 template <int D>

@@ -62,12 +62,13 @@ struct RelArgs {
   float* doff;                // [NH][B][tiles][2 * far + 1], tiles = rel_tiles(S)
   __bf16* dtable;             // [buckets][NH]
   float* dkv;                 // [parts][B][NKV][S][dK, dV] where parts > 1
-  int B, S, NH, NKV, D, width, buckets, far, causal, parts;
+  int B, S, NH, NKV, D, width, buckets, far, causal;
+  int parts, spans;           // workgroups for a tile of keys; spans of the queries among them
   float scale;
 };
 #define GA_REL_TILE 128  // queries a workgroup
 __host__ __device__ inline int rel_tiles(int S) { return (S + GA_REL_TILE - 1) / GA_REL_TILE; }
-int rel_parts(int B, int S, int NH, int NKV);
+void rel_parts(int B, int S, int NH, int NKV, int D, int* parts, int* spans);
 hipError_t rel_forward(const RelArgs& a, hipStream_t s);
 hipError_t rel_backward(const RelArgs& a, hipStream_t s);
 

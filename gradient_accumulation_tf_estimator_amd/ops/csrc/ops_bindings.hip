@@ -383,7 +383,7 @@ std::vector<at::Tensor> rel_attn_bwd(at::Tensor dout, at::Tensor qkv, at::Tensor
   }
   auto dsum = at::empty({a.B, NH, a.S}, lse.options());
   auto doff = at::empty({(int64_t)a.B * NH * rel_tiles(a.S), 2 * a.far + 1}, lse.options());
-  a.parts = rel_parts(a.B, a.S, a.NH, a.NKV);
+  rel_parts(a.B, a.S, a.NH, a.NKV, a.D, &a.parts, &a.spans);
   at::Tensor dkv;
   if (a.parts > 1) {
     dkv = at::empty({(int64_t)a.parts * a.B * NKV * a.S, 2 * a.D}, lse.options());

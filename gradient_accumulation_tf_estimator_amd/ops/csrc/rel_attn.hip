@@ -818,6 +818,7 @@ __global__ __launch_bounds__(64 * kv_waves<D>(), D == 64 ? 3 : 2) void k_rel_bwd
   int tile;
   const int column = place(blockIdx.x - a.NH, a.B * a.NKV, a.parts, tiles, a.causal || a.mask, tile);  // the first tile has the most queries, and keys that count
   const int part = column % a.parts, bk = column / a.parts;
+  const int heads = a.parts / a.spans, part_h = part % heads, span = part / heads;  // every heads-th query head, a span of the queries
   const int hk = bk % a.NKV, b = bk / a.NKV, group = a.NH / a.NKV;
   const int lane = threadIdx.x & 63, hi = lane >> 5;
   const int row = (threadIdx.x >> 6) * 32 + (lane & 31);  // of the tile's keys
@@ -825,7 +826,8 @@ __global__ __launch_bounds__(64 * kv_waves<D>(), D == 64 ? 3 : 2) void k_rel_bwd
   const bool keep = j < a.S && (!a.mask || a.mask[(long long)b * a.S + min(j, a.S - 1)]);
   const bool work = __any(keep);  // this wave has a key that counts
 
-  const int first = a.causal ? tile * KEYS / KC : 0, chunks = (a.S + KC - 1) / KC;
+  const int from = a.causal ? tile * KEYS / KC : 0, chunks = (a.S + KC - 1) / KC - from;
+  const int first = from + chunks * span / a.spans, end = from + chunks * (span + 1) / a.spans;
   Stage<D, T> st;
   st.init(a.width, a.NH * D);
   float row_lse = 0.f, row_d = 0.f;
@@ -864,7 +866,7 @@ __global__ __launch_bounds__(64 * kv_waves<D>(), D == 64 ? 3 : 2) void k_rel_bwd
     fetch(first);
     return Bias<T, true>(a, h);
   };
-  auto next = begin(part);
+  auto next = begin(part_h);
 
   b8 k[D / 16], v[V_LDS ? 1 : D / 16];
   {
@@ -886,8 +888,8 @@ __global__ __launch_bounds__(64 * kv_waves<D>(), D == 64 ? 3 : 2) void k_rel_bwd
   st.wait();
 
   if (__syncthreads_or(work))
-    for (int n = part; n < group; n += a.parts) {
-      if (n != part) {
+    for (int n = part_h; n < group; n += heads) {
+      if (n != part_h) {
         __syncthreads();  // the last head's tiles are read
         next = begin(n);
       }
@@ -895,9 +897,9 @@ __global__ __launch_bounds__(64 * kv_waves<D>(), D == 64 ? 3 : 2) void k_rel_bwd
       put(first);
       __syncthreads();
       const float low = shared(bias[0]), high = shared(bias[2 * a.far + 7]);
-      for (int c = first; c < chunks; ++c) {
+      for (int c = first; c < end; ++c) {
         if (c > first) __syncthreads();
-        if (c + 1 < chunks) fetch(c + 1);
+        if (c + 1 < end) fetch(c + 1);
         const char* qt = buf + (c & 1) * 2 * MAT;
         const char* gt = qt + MAT;
         const float* rl = rows + (c & 1) * 2 * KC;
@@ -945,7 +947,7 @@ __global__ __launch_bounds__(64 * kv_waves<D>(), D == 64 ? 3 : 2) void k_rel_bwd
             }
           }
         }
-        if (c + 1 < chunks) put(c + 1);
+        if (c + 1 < end) put(c + 1);
       }
     }
   // a masked key's column holds what its zeroed K and V gave: it has no gradient
@@ -1252,13 +1254,21 @@ hipError_t token(const RelTokenArgs& a, hipStream_t s) {
 // Over how many workgroups the query heads that share a key/value head are
 // spread in the backward: one workgroup walks all queries of its heads, so
 // with few of them (and uneven ones, under the causal mask) the chip waits for
-// the longest.
-int rel_parts(int B, int S, int NH, int NKV) {
+// the longest. Where that leaves compute units without one, the queries are cut
+// into spans too, of at least four chunks: 1x4000, 2 heads, D 128 222 -> 57 us and
+// 12 for k_rel_dkv, 2x1042 causal, 4 heads, D 128 66 -> 38 and 9, 1x512, 8 heads,
+// D 64 23 -> 18 and 4.
+void rel_parts(int B, int S, int NH, int NKV, int D, int* parts, int* spans) {
   const int group = NH / NKV, tiles = rel_tiles(S);
   int n = 1;
   while (n < group && (long long)B * NKV * tiles * n < 1024) ++n;
   while (group % n) ++n;
-  return n;
+  const int keys = D == 64 ? 32 * kv_waves<64>() : 32 * kv_waves<128>();
+  const long long base = (long long)B * NKV * n * ((S + keys - 1) / keys);
+  int m = 1;
+  while (base * (m + 1) <= 256 && (S + KC - 1) / KC >= 4 * (m + 1)) ++m;
+  *parts = n * m;
+  *spans = m;
 }
 
 // Enough workgroups to fill the chip, but at least 64 keys a wave, since a second

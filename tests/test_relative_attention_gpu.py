@@ -528,3 +528,11 @@ def test_token_long_caches_of_different_lengths():
     B, S, NH, NKV, D = 6, 9000, 4, 2, 64
     lengths = torch.tensor([9000, 1, 4097, 0, 8191, 260], dtype=torch.int32, device="cuda")
     check_token(rand(B, 2, NH, D), rand(B, S, NKV, D), rand(B, S, NKV, D), rand(32, NH), m, lengths)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("B,S,NH,NKV", [(1, 1031, 1, 1), (1, 640, 4, 2), (2, 777, 6, 2)])
+def test_queries_cut_into_spans(B, S, NH, NKV, causal, D):
+    torch.manual_seed(19)
+    check(B, S, NH, NKV, D, causal, padded(B, S, 300) if B > 1 else None)

@@ -55,19 +55,26 @@ struct RelArgs {
   __bf16* out;                // [B][S][NH][D]
   float* lse;                 // [2][B][NH][S]: base 2, +inf for a row with nothing allowed; a factor of P, 1 for
                               // ordinary rows
+  float* split;               // [spans][B][NH][S] of D outputs, then of maximum and sum, where spans > 1
   // backward
   const __bf16* dout;         // [B][S][NH][D]
   float* dsum;                // [B][NH][S]
   __bf16* dqkv;               // like qkv
-  float* doff;                // [NH][B][tiles][2 * far + 1], tiles = rel_tiles(S)
+  float* dq;                  // [q_spans][B][NH][S] of D, then of the row's four sums, where q_spans > 1
+  float* doff;                // [NH][B][rel_doff_rows][2 * far + 1]
   __bf16* dtable;             // [buckets][NH]
   float* dkv;                 // [parts][B][NKV][S][dK, dV] where parts > 1
   int B, S, NH, NKV, D, width, buckets, far, causal;
-  int parts, spans;           // workgroups for a tile of keys; spans of the queries among them
+  int parts, spans;           // backward: workgroups for a tile of keys, spans of the queries among them;
+                              // forward: spans of the keys
+  int q_spans;                // backward: spans of the keys in dQ
   float scale;
 };
 #define GA_REL_TILE 128  // queries a workgroup
 __host__ __device__ inline int rel_tiles(int S) { return (S + GA_REL_TILE - 1) / GA_REL_TILE; }
+// a row of offsets' sums for each tile and span, and one for what joining the spans adds
+__host__ __device__ inline int rel_doff_rows(int S, int q_spans) { return rel_tiles(S) * (q_spans > 1 ? q_spans + 1 : 1); }
+int rel_spans(int B, int S, int NH);
 void rel_parts(int B, int S, int NH, int NKV, int D, int* parts, int* spans);
 hipError_t rel_forward(const RelArgs& a, hipStream_t s);
 hipError_t rel_backward(const RelArgs& a, hipStream_t s);

@@ -359,6 +359,12 @@ std::vector<at::Tensor> rel_attn_fwd(at::Tensor qkv, int64_t NH, int64_t NKV, at
   if (out.numel() == 0) return {out, lse};
   a.out = (__bf16*)out.data_ptr();
   a.lse = want_lse ? lse.data_ptr<float>() : nullptr;
+  a.spans = rel_spans(a.B, a.S, a.NH);
+  at::Tensor split;
+  if (a.spans > 1) {
+    split = at::empty({(int64_t)a.spans * a.B * NH * a.S * (a.D + 2)}, qkv.options().dtype(at::kFloat));
+    a.split = split.data_ptr<float>();
+  }
   check_launch(rel_forward(a, stream_of(qkv)), "rel_attn_fwd");
   return {out, lse};
 }
@@ -382,7 +388,13 @@ std::vector<at::Tensor> rel_attn_bwd(at::Tensor dout, at::Tensor qkv, at::Tensor
     return {dqkv, dtable};
   }
   auto dsum = at::empty({a.B, NH, a.S}, lse.options());
-  auto doff = at::empty({(int64_t)a.B * NH * rel_tiles(a.S), 2 * a.far + 1}, lse.options());
+  a.q_spans = rel_spans(a.B, a.S, a.NH);
+  auto doff = at::empty({(int64_t)a.B * NH * rel_doff_rows(a.S, a.q_spans), 2 * a.far + 1}, lse.options());
+  at::Tensor dq;
+  if (a.q_spans > 1) {
+    dq = at::empty({(int64_t)a.q_spans * a.B * NH * a.S * (a.D + 4)}, lse.options());
+    a.dq = dq.data_ptr<float>();
+  }
   rel_parts(a.B, a.S, a.NH, a.NKV, a.D, &a.parts, &a.spans);
   at::Tensor dkv;
   if (a.parts > 1) {

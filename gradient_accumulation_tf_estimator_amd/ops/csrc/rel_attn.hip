@@ -47,6 +47,7 @@ typedef __attribute__((ext_vector_type(8))) __bf16 b8;
 typedef __attribute__((ext_vector_type(4))) __bf16 b4;
 typedef __attribute__((ext_vector_type(4))) short s4;
 typedef __attribute__((ext_vector_type(8))) short s8;
+typedef __attribute__((ext_vector_type(2))) float f2;
 typedef __attribute__((ext_vector_type(4))) float f4;
 typedef __attribute__((ext_vector_type(16))) float f16;
 typedef __attribute__((address_space(3))) s4 lds_s4;
@@ -145,12 +146,14 @@ struct Stage {
       ay[i] = 2u * (row(i) * sy + col(i));
     }
   }
-  __device__ __forceinline__ static void move(const char* from, unsigned at, const char* to) {
-    const unsigned lds = __builtin_amdgcn_readfirstlane((unsigned)(size_t)(lds_char*)to);
+  __device__ __forceinline__ static void move(const char* from, unsigned at, unsigned to) {
+    extern __shared__ __align__(16) char smem[];
+    const unsigned lds = __builtin_amdgcn_readfirstlane((unsigned)(size_t)(lds_char*)smem + to);
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(at), "s"(from) : "memory");
   }
-  // rows r0 .. r0 + 63 of matrices with row strides sx, sy; rows from `end` on repeat the last one
-  __device__ __forceinline__ void load(const __bf16* px, int sx, const __bf16* py, int sy, int r0, int end, char* tx, char* ty) {
+  // rows r0 .. r0 + 63 of matrices with row strides sx, sy to tiles tx, ty bytes behind the kernel's LDS; rows from
+  // `end` on repeat the last one
+  __device__ __forceinline__ void load(const __bf16* px, int sx, const __bf16* py, int sy, int r0, int end, unsigned tx, unsigned ty) {
     const char* bx = (const char*)(px + (long long)r0 * sx);
     const char* by = (const char*)(py + (long long)r0 * sy);
     const int wave = (threadIdx.x >> 6) * 1024;
@@ -384,6 +387,14 @@ __device__ __forceinline__ void store_rows(char* tile, __bf16* to, long long str
   __builtin_amdgcn_wave_barrier();
 }
 
+// P = exp2(s - lse) * rest. A large maximum (a large bias that all keys of the row
+// share) has no bits left for the sum's logarithm: the sum stays apart.
+__device__ __forceinline__ void save_lse(float* lse, long long rows, float m, float l) {
+  const bool apart = fabsf(m) >= LARGE && l != 0.f;
+  lse[0] = l == 0.f ? INF : apart ? m : m + __builtin_amdgcn_logf(l);
+  lse[rows] = apart ? 1.f / l : 1.f;
+}
+
 // ---------------- forward: a wave owns 32 queries, chunks of 64 keys ----------------
 // padded 24 us (matrix unit 22 % busy), long 163 us (46 %, 841 TFLOP/s)
 template <int D>
@@ -395,7 +406,8 @@ __global__ __launch_bounds__(256, 2) void k_rel_fwd(RelArgs a, int tiles) {
   int* ends = (int*)(bias + 4 * bias_len(a.far));
 
   int tile;
-  const int bh = place(blockIdx.x, a.B * a.NKV, a.NH / a.NKV, tiles, a.causal, tile);
+  const int column = place(blockIdx.x, a.B * a.NKV, a.NH / a.NKV * a.spans, tiles, a.causal, tile);
+  const int bh = column / a.spans, span = column % a.spans;  // a span of the keys
   const int h = bh % a.NH, b = bh / a.NH, hk = h / (a.NH / a.NKV);
   if (a.causal) tile = tiles - 1 - tile;  // the last tile has the most keys
   const int lane = threadIdx.x & 63, hi = lane >> 5;
@@ -411,7 +423,7 @@ __global__ __launch_bounds__(256, 2) void k_rel_fwd(RelArgs a, int tiles) {
   unsigned long long bits = 0, next = 0;
   int key = 0;
   auto fetch = [&](int c) {
-    char* to = buf + (c & 1) * 2 * MAT;
+    const unsigned to = (c & 1) * 2 * MAT;
     key = key_byte(mask, c * KC, end);
     st.load(k, a.width, v, a.width, c * KC, end, to, to + MAT);
   };
@@ -422,17 +434,18 @@ __global__ __launch_bounds__(256, 2) void k_rel_fwd(RelArgs a, int tiles) {
     st.clear(to, to + MAT, next);
   };
   // everything that the first chunk needs is on its way at once
-  fetch(0);
+  const int all = (end + KC - 1) / KC, first = __builtin_amdgcn_readfirstlane(all * span / a.spans);
+  fetch(first);
   const Bias<> first_bias(a, h);
   if (mask) end = mask_end(mask, end, ends);
-  const int chunks = (end + KC - 1) / KC;
+  const int chunks = min((end + KC - 1) / KC, all * (span + 1) / a.spans);
   b8 q[D / 16];
   const __bf16* qp = a.qkv + ((long long)b * a.S + min(i, a.S - 1)) * a.width + h * D;
 #pragma unroll
   for (int t = 0; t < D / 16; ++t) q[t] = *(const b8*)(qp + 16 * t + 8 * hi);
   first_bias.put(a.scale, bias);
   st.wait();
-  if (chunks > 0) arrive(0);
+  if (first < chunks) arrive(first);
   __syncthreads();
 
   f16 o[D / 32] = {};
@@ -441,9 +454,9 @@ __global__ __launch_bounds__(256, 2) void k_rel_fwd(RelArgs a, int tiles) {
   const float low = shared(bias[0]), high = shared(bias[2 * a.far + 7]);
   const Flat flat_low(low, c2), flat_high(high, c2);
 
-  for (int c = 0; c < chunks; ++c) {
+  for (int c = first; c < chunks; ++c) {
     bits = next;
-    if (c > 0) __syncthreads();
+    if (c > first) __syncthreads();
     if (c + 1 < chunks) fetch(c + 1);
     const char* kt = buf + (c & 1) * 2 * MAT;
     const char* vt = kt + MAT;
@@ -515,17 +528,44 @@ __global__ __launch_bounds__(256, 2) void k_rel_fwd(RelArgs a, int tiles) {
     if (c + 1 < chunks) arrive(c + 1);
   }
   l += __shfl_xor(l, 32, 64);
+  if (a.spans > 1) {
+    if (i >= a.S) return;
+    const long long rows = (long long)a.B * a.NH * a.S, row = span * rows + (long long)bh * a.S + i;
+    store_columns<D>(a.split + row * D, o, 1.f, hi);
+    if (hi == 0) *(f2*)(a.split + a.spans * rows * D + row * 2) = f2{m, l};
+    return;
+  }
   __syncthreads();  // the tiles are read
   store_rows<D>(smem + (threadIdx.x >> 6) * 64 * D, a.out + (((long long)b * a.S + i0) * a.NH + h) * D, a.NH * D, a.S - i0, o,
                 l == 0.f ? 0.f : 1.f / l, lane);
-  if (i < a.S && a.lse && hi == 0) {
-    // P = exp2(s - lse) * rest. A large maximum (a large bias that all keys of the
-    // row share) has no bits left for the sum's logarithm: the sum stays apart.
-    const bool apart = fabsf(m) >= LARGE && l != 0.f;
-    float* lse = a.lse + (long long)bh * a.S + i;
-    lse[0] = l == 0.f ? INF : apart ? m : m + __builtin_amdgcn_logf(l);
-    lse[(long long)a.B * a.NH * a.S] = apart ? 1.f / l : 1.f;
+  if (i < a.S && a.lse && hi == 0) save_lse(a.lse + (long long)bh * a.S + i, (long long)a.B * a.NH * a.S, m, l);
+}
+
+// joins the spans of a row, in order: four columns a thread (4 to 6 us at up to 32768 rows)
+template <int D>
+__global__ __launch_bounds__(256) void k_rel_out(RelArgs a) {
+  const long long rows = (long long)a.B * a.NH * a.S, row = (long long)blockIdx.x * (1024 / D) + threadIdx.x / (D / 4);
+  const int d = threadIdx.x % (D / 4) * 4;
+  if (row >= rows) return;
+  const float* ml = a.split + a.spans * rows * D;
+  float m = -INF, l = 0.f;
+  for (int s = 0; s < a.spans; ++s) m = larger(m, ml[(s * rows + row) * 2]);
+  const float base = m == -INF ? 0.f : m;
+  f4 o = {};
+  for (int s = 0; s < a.spans; ++s) {
+    const f2 x = *(const f2*)(ml + (s * rows + row) * 2);
+    const float f = __builtin_amdgcn_exp2f(x[0] - base);
+    l = fmaf(x[1], f, l);
+    o += *(const f4*)(a.split + (s * rows + row) * D + d) * f;
   }
+  const int i = (int)(row % a.S), h = (int)(row / a.S % a.NH);
+  const long long b = row / a.S / a.NH;
+  const float f = l == 0.f ? 0.f : 1.f / l;
+  b4 v;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = (__bf16)(o[e] * f);
+  *(b4*)(a.out + ((b * a.S + i) * a.NH + h) * D + d) = v;
+  if (a.lse && d == 0) save_lse(a.lse + row, rows, m, l);
 }
 
 // lane i of each 16 takes lane i + N's value (N < 0: i - |N|), zero from outside
@@ -570,7 +610,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_rel_bwd_q(RelArgs a, i
   float* sums = (float*)(ends + 4);  // [4 waves][2 halves][offs]
 
   int tile;
-  const int bh = place(blockIdx.x, a.B * a.NKV, a.NH / a.NKV, tiles, a.causal, tile);
+  const int column = place(blockIdx.x, a.B * a.NKV, a.NH / a.NKV * a.q_spans, tiles, a.causal, tile);
+  const int bh = column / a.q_spans, span = column % a.q_spans;  // a span of the keys
   const int h = bh % a.NH, b = bh / a.NH, hk = h / (a.NH / a.NKV);
   if (a.causal) tile = tiles - 1 - tile;  // the last tile has the most keys
   const int lane = threadIdx.x & 63, hi = lane >> 5, wave = threadIdx.x >> 6;
@@ -586,7 +627,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_rel_bwd_q(RelArgs a, i
   unsigned long long bits = 0, next = 0;
   int key = 0;
   auto fetch = [&](int c) {
-    char* to = buf + (c & 1) * 2 * MAT;
+    const unsigned to = (c & 1) * 2 * MAT;
     key = key_byte(mask, c * KC, end);
     st.load(k, a.width, v, a.width, c * KC, end, to, to + MAT);
   };
@@ -597,10 +638,11 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_rel_bwd_q(RelArgs a, i
     st.clear(to, to + MAT, next);
   };
   // everything that the first chunk needs is on its way at once
-  fetch(0);
+  const int all = (end + KC - 1) / KC, first = __builtin_amdgcn_readfirstlane(all * span / a.q_spans);
+  fetch(first);
   const Bias<> first_bias(a, h);
   if (mask) end = mask_end(mask, end, ends);
-  const int chunks = (end + KC - 1) / KC;
+  const int chunks = min((end + KC - 1) / KC, all * (span + 1) / a.q_spans);
   // a row past the end, or with nothing allowed, takes part as zeros
   const float lse = i < a.S ? a.lse[(long long)bh * a.S + i] : INF;
   const float rest_p = a.lse[(long long)a.B * a.NH * a.S + (long long)bh * a.S + min(i, a.S - 1)];  // 1, or 1 / sum
@@ -624,7 +666,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_rel_bwd_q(RelArgs a, i
     }
   }
   dsum += __shfl_xor(dsum, 32, 64);
-  if (i < a.S && hi == 0) a.dsum[(long long)bh * a.S + i] = dsum;
+  if (i < a.S && hi == 0 && span == 0) a.dsum[(long long)bh * a.S + i] = dsum;
 
   f16 dq[D / 32] = {};
   const float c2 = a.scale * LOG2E;
@@ -652,15 +694,15 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_rel_bwd_q(RelArgs a, i
   first_bias.put(a.scale, bias);
   for (int x = threadIdx.x; x < 8 * offs; x += 256) sums[x] = 0.f;
   st.wait();
-  if (chunks > 0) arrive(0);
+  if (first < chunks) arrive(first);
   __syncthreads();
   const float low = shared(bias[0]), high = shared(bias[2 * a.far + 7]);
   const Flat flat_low(low, c2), flat_high(high, c2);
   dsum *= rest_p;
 
-  for (int c = 0; c < chunks; ++c) {
+  for (int c = first; c < chunks; ++c) {
     bits = next;
-    if (c > 0) __syncthreads();
+    if (c > first) __syncthreads();
     if (c + 1 < chunks) fetch(c + 1);
     const char* kt = buf + (c & 1) * 2 * MAT;
     const char* vt = kt + MAT;
@@ -730,8 +772,20 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_rel_bwd_q(RelArgs a, i
   }
   add(left_at - i0 + lane_off, left);
   rest += __shfl_xor(rest, 32, 64);
-  far_low += fmaf(-rest, mass_low * rest_p, own_low);  // each half takes its own share
-  far_high += fmaf(-rest, mass_high * rest_p, own_high);
+  mass_low *= rest_p;
+  mass_high *= rest_p;
+  if (a.q_spans > 1) {  // the row's sums are known to k_rel_dq
+    const long long rows = (long long)a.B * a.NH * a.S, row = span * rows + (long long)bh * a.S + i;
+    mass_low += __shfl_xor(mass_low, 32, 64);
+    mass_high += __shfl_xor(mass_high, 32, 64);
+    if (i < a.S) {
+      store_columns<D>(a.dq + row * D, dq, a.scale, hi);
+      if (hi == 0) *(f4*)(a.dq + a.q_spans * rows * D + row * 4) = f4{rest, mass_low, mass_high, 0.f};
+    }
+    rest = 0.f;
+  }
+  far_low += fmaf(-rest, mass_low, own_low);  // each half takes its own share
+  far_high += fmaf(-rest, mass_high, own_high);
 #pragma unroll
   for (int x = 32; x > 0; x >>= 1) {
     far_low += __shfl_xor(far_low, x, 64);
@@ -742,14 +796,62 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_rel_bwd_q(RelArgs a, i
     mine[offs - 1] += far_high;
   }
   __syncthreads();
-  store_rows<D>(smem + wave * 64 * D, a.dqkv + ((long long)b * a.S + i0) * a.width + h * D, a.width, a.S - i0, dq, a.scale, lane);
-  float* to = a.doff + (((long long)h * a.B + b) * tiles + tile) * offs;
+  if (a.q_spans == 1)
+    store_rows<D>(smem + wave * 64 * D, a.dqkv + ((long long)b * a.S + i0) * a.width + h * D, a.width, a.S - i0, dq, a.scale, lane);
+  float* to = a.doff + (((long long)h * a.B + b) * rel_doff_rows(a.S, a.q_spans) + tile * a.q_spans + span) * offs;
   for (int x = threadIdx.x; x < offs; x += 256) {
     float t = 0.f;
 #pragma unroll
     for (int n = 0; n < 8; ++n) t += sums[n * offs + x];
     to[x] = t;
   }
+}
+
+// Joins the spans: dQ, four columns a thread, in order; and in the first workgroups,
+// one for 128 rows, what the rows' sums take out of the two outermost offsets, as
+// one more row of offsets' sums (5.5 us).
+template <int D>
+__global__ __launch_bounds__(256) void k_rel_dq(RelArgs a, int tiles) {
+  __shared__ float lds[2][2];
+  const long long rows = (long long)a.B * a.NH * a.S;
+  const int sums = a.B * a.NH * tiles;
+  if ((int)blockIdx.x >= sums) {
+    const long long row = (long long)(blockIdx.x - sums) * (1024 / D) + threadIdx.x / (D / 4);
+    const int d = threadIdx.x % (D / 4) * 4;
+    if (row >= rows) return;
+    f4 t = {};
+    for (int s = 0; s < a.q_spans; ++s) t += *(const f4*)(a.dq + (s * rows + row) * D + d);
+    b4 v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = (__bf16)t[e];
+    const int i = (int)(row % a.S), h = (int)(row / a.S % a.NH);
+    const long long b = row / a.S / a.NH;
+    *(b4*)(a.dqkv + (b * a.S + i) * a.width + h * D + d) = v;
+    return;
+  }
+  const int tile = blockIdx.x % tiles, bh = blockIdx.x / tiles, h = bh % a.NH, b = bh / a.NH;
+  const int i = tile * TILE + threadIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  float low = 0.f, high = 0.f;
+  if (threadIdx.x < TILE && i < a.S) {
+    f4 t = {};
+    for (int s = 0; s < a.q_spans; ++s) t += *(const f4*)(a.dq + a.q_spans * rows * D + (s * rows + (long long)bh * a.S + i) * 4);
+    low = -t[0] * t[1];
+    high = -t[0] * t[2];
+  }
+#pragma unroll
+  for (int x = 32; x > 0; x >>= 1) {
+    low += __shfl_xor(low, x, 64);
+    high += __shfl_xor(high, x, 64);
+  }
+  if (lane == 0 && wave < 2) {
+    lds[wave][0] = low;
+    lds[wave][1] = high;
+  }
+  __syncthreads();
+  const int offs = 2 * a.far + 1;
+  float* to = a.doff + (((long long)h * a.B + b) * rel_doff_rows(a.S, a.q_spans) + tiles * a.q_spans + tile) * offs;
+  for (int x = threadIdx.x; x < offs; x += 256)
+    to[x] = x == 0 ? lds[0][0] + lds[1][0] : x == offs - 1 ? lds[0][1] + lds[1][1] : 0.f;
 }
 
 // dtable[n][h]: the offsets' sums over batches and tiles, then over the offsets
@@ -763,7 +865,7 @@ __device__ void sum_table(const RelArgs& a, int h, char* smem) {
   float* sums = part + W * COLS;                             // [2 * far + 1]
   short* map = (short*)(sums + 2 * GA_REL_MAX_DISTANCE + 1);  // [2 * far + 1]
   const int offs = 2 * a.far + 1, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int n = a.B * rel_tiles(a.S);
+  const int n = a.B * rel_doff_rows(a.S, a.q_spans);
   const float* p = a.doff + (long long)h * n * offs;
   for (int x = threadIdx.x; x < offs; x += T) map[x] = (short)min(max(a.map[x], 0), a.buckets - 1);
   for (int x0 = 0; x0 < offs; x0 += COLS) {
@@ -834,7 +936,7 @@ __global__ __launch_bounds__(64 * kv_waves<D>(), D == 64 ? 3 : 2) void k_rel_bwd
   const __bf16 *q, *g;
   const float *lse, *dsum;
   auto fetch = [&](int c) {
-    char* to = buf + (c & 1) * 2 * MAT;
+    const unsigned to = (c & 1) * 2 * MAT;
     const int r = c * KC + lane;
     row_lse = lse[min(r, a.S - 1)];
     row_d = dsum[min(r, a.S - 1)];
@@ -1209,9 +1311,14 @@ template <int D>
 hipError_t forward(const RelArgs& a, hipStream_t s) {
   const int tiles = rel_tiles(a.S);
   const size_t lds = 4 * KC * 2 * D + bias_bytes(a.far) + 16;
-  const hipError_t e = allow(k_rel_fwd<D>, lds);
+  hipError_t e = allow(k_rel_fwd<D>, lds);
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL((k_rel_fwd<D>), dim3(a.B * a.NH * tiles), dim3(256), lds, s, a, tiles);
+  hipLaunchKernelGGL((k_rel_fwd<D>), dim3(a.B * a.NH * tiles * a.spans), dim3(256), lds, s, a, tiles);
+  if ((e = hipGetLastError()) != hipSuccess) return e;
+  if (a.spans > 1) {
+    const long long rows = (long long)a.B * a.NH * a.S;
+    hipLaunchKernelGGL((k_rel_out<D>), dim3((unsigned)((rows + 1024 / D - 1) / (1024 / D))), dim3(256), 0, s, a);
+  }
   return hipGetLastError();
 }
 
@@ -1225,8 +1332,13 @@ hipError_t backward(const RelArgs& a, hipStream_t s) {
   hipError_t e = allow(k_rel_bwd_q<D>, lds_q);
   if (e == hipSuccess) e = allow(k_rel_bwd_kv<D>, lds_kv);
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL((k_rel_bwd_q<D>), dim3(a.B * a.NH * tiles), dim3(256), lds_q, s, a, tiles);
+  hipLaunchKernelGGL((k_rel_bwd_q<D>), dim3(a.B * a.NH * tiles * a.q_spans), dim3(256), lds_q, s, a, tiles);
   if ((e = hipGetLastError()) != hipSuccess) return e;
+  if (a.q_spans > 1) {
+    const long long rows = (long long)a.B * a.NH * a.S;
+    hipLaunchKernelGGL((k_rel_dq<D>), dim3((unsigned)(a.B * a.NH * tiles + (rows + 1024 / D - 1) / (1024 / D))), dim3(256), 0, s, a, tiles);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+  }
   hipLaunchKernelGGL((k_rel_bwd_kv<D>), dim3(a.NH + a.B * a.NKV * a.parts * kv_tiles), dim3(T), lds_kv, s, a, kv_tiles);
   if ((e = hipGetLastError()) != hipSuccess) return e;
   if (a.parts > 1) {
@@ -1250,6 +1362,18 @@ hipError_t token(const RelTokenArgs& a, hipStream_t s) {
 }
 
 }  // namespace
+
+// Over how many workgroups the keys of a tile of queries are cut where there are
+// few tiles, of at least five chunks each. With their joining kernels, forward and
+// dQ: 1x4000, 2 heads, D 128 88 -> 38 and 147 -> 57 us; 2x1042 causal, 4 heads, D 128
+// 28 -> 22 and 44 -> 32; 1x2000, 8 heads, D 64 37 -> 28 and 62 -> 46. In two spans of
+// four chunks 1x512 would lose (13 -> 14 and 22 -> 23).
+int rel_spans(int B, int S, int NH) {
+  const long long base = (long long)B * NH * rel_tiles(S);
+  int n = 1;
+  while (base * (n + 1) <= 256 && (S + KC - 1) / KC >= 5 * (n + 1)) ++n;
+  return n;
+}
 
 // Over how many workgroups the query heads that share a key/value head are
 // spread in the backward: one workgroup walks all queries of its heads, so

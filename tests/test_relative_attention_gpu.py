@@ -536,3 +536,72 @@ def test_token_long_caches_of_different_lengths():
 def test_queries_cut_into_spans(B, S, NH, NKV, causal, D):
     torch.manual_seed(19)
     check(B, S, NH, NKV, D, causal, padded(B, S, 300) if B > 1 else None)
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("kind", ["empty", "holes", "left", "late"])
+def test_masks_over_spans(kind, causal):
+    """Keys cut over several workgroups, some of which find none that counts."""
+    torch.manual_seed(20)
+    B, S = 2, 700
+    mask = padded(B, S, 90)
+    if kind == "empty":
+        mask[0] = 0
+    elif kind == "holes":
+        mask = (torch.rand(B, S, device="cuda") < 0.2).to(torch.uint8)
+    elif kind == "left":
+        mask = mask.flip(1).contiguous()
+    elif kind == "late":
+        mask = torch.zeros(B, S, dtype=torch.uint8, device="cuda")
+        mask[:, 650:] = 1
+    check(B, S, 2, 1, 64, causal, mask, poison=True)
+
+
+@pytest.mark.parametrize("value", [-(2.0**20), 99614720.0])
+def test_one_large_bias_over_spans(value):
+    """As test_one_large_bias_for_all, for out and dv of a batch whose keys and queries are cut."""
+    torch.manual_seed(21)
+    S, NH, D = 1100, 2, 64
+    m = relative_position_buckets(32, 128).cuda()
+    qkv = rand(1, S, 3 * NH * D)
+    qkv[:, :, :2 * NH * D] *= 2.0**-8
+    dout = rand(1, S, NH * D)
+    leaf, table = qkv.clone().requires_grad_(), torch.full((32, NH), value, device="cuda").bfloat16()
+    out = fused_relative_attention(leaf, NH, table, m)
+    dv = torch.autograd.grad(out, leaf, dout)[0].double().view(1, S, 3, NH, D)[:, :, 2].transpose(1, 2)
+    q, k, v = split(qkv, NH, NH)
+    keep = torch.ones(1, 1, S, S, dtype=torch.bool, device="cuda")
+    p, r = probabilities(q, k, torch.zeros(1, NH, S, S, device="cuda", dtype=torch.float64), keep, D ** -0.5)
+    r += 2.1 * float((q @ k.transpose(2, 3).contiguous()).abs().amax()) * D ** -0.5
+    do = dout.double().view(1, S, NH, D).transpose(1, 2).contiguous()
+    pt = p.transpose(2, 3).contiguous()
+    for got, want, tol in ((out.detach().double().view(1, S, NH, D).transpose(1, 2), p @ v, (2 * U + 2 * r) * (p @ v.abs())),
+                           (dv, pt @ do, (2 * U + 2 * r + S * E32) * (pt @ do.abs()))):
+        assert ((got - want).abs() <= tol * (1 + U) + U * want.abs() + 1e-30).all()
+
+
+def test_spans_captured_and_repeated():
+    """The spans' workspaces inside a graph: every replay is the eager result, bit for bit."""
+    torch.manual_seed(22)
+    m = relative_position_buckets(32, 128, False).cuda()
+    qkv, table, dout = rand(1, 900, 4 * 64).requires_grad_(), rand(32, 2).requires_grad_(), rand(1, 900, 128)
+
+    def step():
+        out = fused_relative_attention(qkv, 2, table, m, nkv=1, causal=True)
+        return [out.detach(), *torch.autograd.grad(out, (qkv, table), dout)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for _ in range(3):
+        with torch.no_grad():
+            qkv.normal_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, step()))

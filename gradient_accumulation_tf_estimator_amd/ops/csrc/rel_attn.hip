@@ -396,7 +396,7 @@ __device__ __forceinline__ void save_lse(float* lse, long long rows, float m, fl
 }
 
 // ---------------- forward: a wave owns 32 queries, chunks of 64 keys ----------------
-// padded 24 us (matrix unit 22 % busy), long 163 us (46 %, 841 TFLOP/s)
+// padded 24 us (matrix unit 22 % busy), long 163 us (47 %, 841 TFLOP/s)
 template <int D>
 __global__ __launch_bounds__(256, 2) void k_rel_fwd(RelArgs a, int tiles) {
   extern __shared__ __align__(16) char smem[];  // the tiles lie in the first 64 KB, which m0 reaches
@@ -598,7 +598,7 @@ __device__ __forceinline__ void diagonals_32(const f16& c, float* d, bool ib) {
 }
 
 // ---------------- backward 1: dQ, D and the offsets' sums of dS ----------------
-// padded 38 us (matrix unit 19 % busy), long 243 us (42 %, 848 TFLOP/s)
+// padded 38 us (matrix unit 19 % busy), long 243 us (43 %, 848 TFLOP/s)
 template <int D>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_rel_bwd_q(RelArgs a, int tiles) {
   extern __shared__ __align__(16) char smem[];  // the tiles lie in the first 64 KB, which m0 reaches
@@ -901,7 +901,7 @@ __device__ void sum_table(const RelArgs& a, int h, char* smem) {
 // 128. V is kept in LDS there, by eight waves that share a chunk instead of four:
 // two waves a SIMD (long: 480 us with V in registers, 340 so, when that step was
 // taken; padded: 45 us with V in registers, 61 in LDS with four waves, 85 with
-// eight). padded 44 us (matrix unit 21 % busy), long 297 us (43 %, 925 TFLOP/s),
+// eight). padded 43 us (matrix unit 22 % busy), long 297 us (43 %, 925 TFLOP/s),
 // the table's sums among them.
 template <int D>
 constexpr int kv_waves() { return D == 64 ? 4 : 8; }

@@ -327,7 +327,7 @@ RelArgs rel_args(const at::Tensor& qkv, int64_t NH, int64_t NKV, const at::Tenso
   TORCH_CHECK(scale > 0 && std::isfinite(scale), "scale must be positive and finite");
   // a launch has fewer than 2^32 threads, 512 for each 128 rows of a head; a chunk of 64 rows is addressed by 32 bits from its start
   TORCH_CHECK(qkv.size(2) <= (1 << 23), "too many heads");
-  TORCH_CHECK(S < (1ll << 24) && B * NH * (S / 128 + 1) < (1ll << 23), "too many rows");
+  TORCH_CHECK(S < (1ll << 24) && B * NH * (S / 128 + 1) < (1ll << 22), "too many rows");
   if (mask)
     TORCH_CHECK(mask->device() == qkv.device() && mask->scalar_type() == at::kByte && mask->is_contiguous() &&
                 mask->dim() == 2 && mask->size(0) == B && mask->size(1) == S, "mask must be a contiguous u8 [B, S] tensor");
@@ -467,7 +467,8 @@ at::Tensor rel_attn_token(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor t
               lengths.dim() == 1 && lengths.numel() == B, "lengths must be an int32 [B] tensor on the same GPU");
   TORCH_CHECK(scale > 0 && std::isfinite(scale), "scale must be positive and finite");
   TORCH_CHECK(NH / NKV <= 32, "at most 32 query heads a key/value head");
-  TORCH_CHECK(S < (1ll << 31) - 64 && B * NH * Sq < (1ll << 24), "too many rows");
+  // fewer than 2^32 threads here too
+  TORCH_CHECK(S < (1ll << 31) - 64 && B * NH * Sq < (1ll << 22), "too many rows");
   const c10::OptionalDeviceGuard guard(q.device());
   auto out = at::empty({B, Sq, NH, D}, q.options());
   if (out.numel() == 0) return out;

@@ -605,3 +605,19 @@ def test_spans_captured_and_repeated():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, step()))
+
+
+def test_launches_beyond_the_grid_are_refused():
+    m = relative_position_buckets().cuda()
+    t = rand(32, 1)
+    with pytest.raises(RuntimeError, match="too many rows"):
+        fused_relative_attention(torch.zeros(1 << 22, 1, 192, dtype=torch.bfloat16, device="cuda"), 1, t, m)
+    q, k = rand(1, 1, 1, 64).expand(1 << 22, 1, 1, 64), rand(1, 4, 1, 64).expand(1 << 22, 4, 1, 64)
+    with pytest.raises(RuntimeError, match="too many rows"):
+        relative_attention_decode(q, k, k, t, m, torch.ones(1 << 22, dtype=torch.int32, device="cuda"))
+    n = 70000
+    q, k = rand(1, 1, 1, 64).expand(n, 1, 1, 64), rand(1, 4, 1, 64).expand(n, 4, 1, 64)
+    out = relative_attention_decode(q, k, k, t, m, torch.full((n,), 3, dtype=torch.int32, device="cuda"))
+    assert torch.equal(out, out[:1].expand_as(out))
+    out = fused_relative_attention(rand(1, 1, 192).expand(n, 1, 192).contiguous(), 1, t, m)
+    assert torch.equal(out, out[:1].expand_as(out))

@@ -143,6 +143,7 @@ class AccumEngine:
 
             fused_ops.flush_pending_wgrads()
             fused_ops.flush_pending_colreduce()
+            fused_ops.release_held_wgrads()
         st = self.state
         lo, hi = st.layout.grad_lo, st.layout.grad_hi
         if hi <= lo:

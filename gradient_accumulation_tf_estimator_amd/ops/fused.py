@@ -33,6 +33,17 @@ def _use_hip(x: torch.Tensor) -> bool:
 # stream before all-reduce/apply (AccumEngine.apply*).
 _WGRAD_OVERLAP = False
 _wgrad_stream = None
+# Output gradients that the side stream may still be reading. Autograd adds a
+# second branch's gradient into the first's memory, on the main stream, once it
+# holds the last reference (y = residual + linear(x) hands one tensor to both);
+# record_stream keeps that memory from being reused, not from being written. So
+# a reference is kept until the backward is over (AccumEngine.accumulate).
+_wgrad_held = []
+
+
+def release_held_wgrads() -> None:
+    _wgrad_held.clear()
+
 
 # ---- grouped wgrad -----------------------------------------------------
 # Collect the micro-step's wgrads during backward and issue them as ONE
@@ -377,6 +388,7 @@ class _DirectLinearFn(torch.autograd.Function):
                 gemm.wgrad_acc(x2d, dy2d, ctx.module._accum_view_w)
             x2d.record_stream(s)
             dy2d.record_stream(s)
+            _wgrad_held.append(dy)
             if vb is not None:
                 vb.add_(dy2d.sum(0, dtype=torch.float32))
         else:

@@ -28,26 +28,46 @@
                 " at " #expr);                                           \
   } while (0)
 
+namespace {
+
+hipblasLtHandle_t new_handle() {
+  hipblasLtHandle_t h;
+  hipblasStatus_t st = hipblasLtCreate(&h);
+  TORCH_CHECK(st == HIPBLAS_STATUS_SUCCESS, "hipblasLtCreate failed");
+  return h;
+}
+
+void* new_workspace() {
+  void* p = nullptr;
+  TORCH_CHECK(hipMalloc(&p, 64ull << 20) == hipSuccess, "no memory for the GEMM workspace");
+  return p;
+}
+
+}  // namespace
+
 hipblasLtHandle_t ga_lt_handle() {
-  static hipblasLtHandle_t h = [] {
-    hipblasLtHandle_t hh;
-    hipblasStatus_t st = hipblasLtCreate(&hh);
-    TORCH_CHECK(st == HIPBLAS_STATUS_SUCCESS, "hipblasLtCreate failed");
-    return hh;
-  }();
+  static hipblasLtHandle_t h = new_handle();
   return h;
 }
 
 void* ga_lt_workspace() {
-  static void* ws = [] {
-    void* p = nullptr;
-    (void)hipMalloc(&p, 64ull << 20);
-    return p;
-  }();
+  static void* ws = new_workspace();
   return ws;
 }
 
 namespace {
+
+// Products on two streams at once may share neither: a split product leaves its
+// parts in the workspace. The side stream's weight gradients have their own.
+hipblasLtHandle_t side_handle() {
+  static hipblasLtHandle_t h = new_handle();
+  return h;
+}
+
+void* side_workspace() {
+  static void* ws = new_workspace();
+  return ws;
+}
 
 struct LtPlan {
   hipblasLtMatmulDesc_t desc;
@@ -98,9 +118,11 @@ int64_t wgrad_algo_count(int64_t K, int64_t N, int64_t R) {
   return (int64_t)plan_for(K, N, R).algos.size();
 }
 
-// dW accum_slice[N*K fp32] += dy[R,N]^T @ x[R,K]
+// dW accum_slice[N*K fp32] += dy[R,N]^T @ x[R,K]; workspace 1 is the side
+// stream's, 0 everyone else's
 void wgrad_acc(at::Tensor x, at::Tensor dy, at::Tensor accum_slice,
-               int64_t algo_idx) {
+               int64_t algo_idx, int64_t workspace) {
+  TORCH_CHECK(workspace == 0 || workspace == 1, "workspace must be 0 or 1, got ", workspace);
   TORCH_CHECK(x.is_cuda() && x.is_contiguous() && x.scalar_type() == at::kBFloat16,
               "x must be contiguous bf16");
   TORCH_CHECK(dy.is_cuda() && dy.is_contiguous() && dy.scalar_type() == at::kBFloat16,
@@ -119,9 +141,10 @@ void wgrad_acc(at::Tensor x, at::Tensor dy, at::Tensor accum_slice,
   int idx = (int)std::min<int64_t>(std::max<int64_t>(algo_idx, 0),
                                    (int64_t)p.algos.size() - 1);
   HIPBLASLT_CHECK(hipblasLtMatmul(
-      ga_lt_handle(), p.desc, &alpha, x.data_ptr(), p.la, dy.data_ptr(), p.lb,
-      &beta, accum_slice.data_ptr(), p.lc, accum_slice.data_ptr(), p.lc,
-      &p.algos[idx].algo, ga_lt_workspace(), kWorkspaceBytes, stream));
+      workspace ? side_handle() : ga_lt_handle(), p.desc, &alpha, x.data_ptr(),
+      p.la, dy.data_ptr(), p.lb, &beta, accum_slice.data_ptr(), p.lc,
+      accum_slice.data_ptr(), p.lc, &p.algos[idx].algo,
+      workspace ? side_workspace() : ga_lt_workspace(), kWorkspaceBytes, stream));
 }
 
 }  // namespace
@@ -130,6 +153,6 @@ void register_blas_acc(pybind11::module_& mod) {
   mod.def("wgrad_acc", &wgrad_acc,
           "accum_slice[N,K] += dy[R,N]^T @ x[R,K] (bf16 in, fp32 accumulate)",
           pybind11::arg("x"), pybind11::arg("dy"), pybind11::arg("accum_slice"),
-          pybind11::arg("algo_idx") = 0);
+          pybind11::arg("algo_idx") = 0, pybind11::arg("workspace") = 0);
   mod.def("wgrad_algo_count", &wgrad_algo_count);
 }

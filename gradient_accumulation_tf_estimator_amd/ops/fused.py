@@ -385,7 +385,7 @@ class _DirectLinearFn(torch.autograd.Function):
             s = wgrad_stream()
             s.wait_stream(torch.cuda.current_stream())
             with torch.cuda.stream(s):
-                gemm.wgrad_acc(x2d, dy2d, ctx.module._accum_view_w)
+                gemm.wgrad_acc(x2d, dy2d, ctx.module._accum_view_w, gemm.SIDE_WORKSPACE)
             x2d.record_stream(s)
             dy2d.record_stream(s)
             _wgrad_held.append(dy)

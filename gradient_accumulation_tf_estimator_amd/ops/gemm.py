@@ -103,7 +103,10 @@ def dgrad_add(dy2d: torch.Tensor, w: torch.Tensor, addend: torch.Tensor) -> torc
     return hip.lt_dgrad_add(dy2d, w, addend, idx)
 
 
-def wgrad_acc(x2d: torch.Tensor, dy2d: torch.Tensor, accum_2d: torch.Tensor) -> None:
+SIDE_WORKSPACE = 1  # of products on the wgrad side stream; the main stream's, which run beside them, use 0
+
+
+def wgrad_acc(x2d: torch.Tensor, dy2d: torch.Tensor, accum_2d: torch.Tensor, workspace: int = 0) -> None:
     hip = require_hip()
     K = x2d.shape[-1]
     N = dy2d.shape[-1]
@@ -118,9 +121,9 @@ def wgrad_acc(x2d: torch.Tensor, dy2d: torch.Tensor, accum_2d: torch.Tensor) -> 
             # slice is not polluted by tuning runs
             scratch = torch.zeros_like(accum_2d)
             idx = _tune(key, hip.wgrad_algo_count(K, N, R),
-                        lambda i: hip.wgrad_acc(x2d, dy2d, scratch, i))
+                        lambda i: hip.wgrad_acc(x2d, dy2d, scratch, i, workspace))
             del scratch
-    hip.wgrad_acc(x2d, dy2d, accum_2d, idx)
+    hip.wgrad_acc(x2d, dy2d, accum_2d, idx, workspace)
 
 
 def linear_gelu(x2d: torch.Tensor, w: torch.Tensor, bias: torch.Tensor):

@@ -44,3 +44,12 @@ def require_hip():
             f"(import error: {_hip_err})"
         )
     return mod
+
+
+def refuse_tangents(name: str, *tensors) -> None:
+    """For operators without a gradient, on the CPU; the bindings check the
+    same of the kernels' operands."""
+    from torch.autograd import forward_ad
+
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{name} has no gradient, forward-mode ones included")

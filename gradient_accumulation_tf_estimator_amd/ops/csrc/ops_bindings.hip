@@ -139,6 +139,9 @@ void once() {
   TORCH_CHECK(!at::GradMode::is_enabled(), "this operator has no second derivative: call it without create_graph");
 }
 
+// whether a forward-mode derivative comes with the tensor (there is one level)
+bool has_tangent(const at::Tensor& t) { return t._fw_grad(/*level=*/0).defined(); }
+
 // The autograd node lives here: in Python its forward and backward cost more
 // than the kernels on a small batch. `dw_acc`: an fp32 slice that the weight's
 // gradient is added to instead of being returned.
@@ -176,6 +179,8 @@ std::vector<at::Tensor> add_rms_norm(at::Tensor x, MaybeTensor res, at::Tensor w
 
 std::vector<at::Tensor> rms_norm_fp8(at::Tensor x, MaybeTensor res, at::Tensor w, double eps, int64_t group) {
   bool vec;
+  TORCH_CHECK(!has_tangent(x) && !(res && has_tangent(*res)) && !has_tangent(w),
+              "rms_norm_fp8 has no gradient, forward-mode ones included");
   auto shape = x.sizes().vec();  // the outputs have the caller's shape
   const auto given = x;
   x = as_rows(x);
@@ -444,6 +449,7 @@ struct RelAttention : public torch::autograd::Function<RelAttention> {
 // with gradients recorded, the forward keeps what the backward needs
 at::Tensor rel_attention(at::Tensor qkv, at::Tensor table, at::Tensor map, MaybeTensor mask, int64_t NH, int64_t NKV,
                          bool causal, double scale) {
+  TORCH_CHECK(!has_tangent(qkv) && !has_tangent(table), "relative attention has no forward-mode derivative on a GPU");
   if (at::GradMode::is_enabled() && (qkv.requires_grad() || table.requires_grad()))
     return RelAttention::apply(qkv, table, map, mask, NH, NKV, causal, scale);
   return rel_attn_fwd(aligned(qkv), NH, NKV, table.contiguous(), map, mask, causal, scale, false)[0];
@@ -452,6 +458,8 @@ at::Tensor rel_attention(at::Tensor qkv, at::Tensor table, at::Tensor map, Maybe
 // q [B, Sq, NH, D], caches [B, S, NKV, D] of any strides with contiguous, 16-byte aligned rows
 at::Tensor rel_attn_token(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor table, at::Tensor map,
                           at::Tensor lengths, double scale) {
+  for (const auto& t : {q, k, v, table})
+    TORCH_CHECK(!has_tangent(t), "relative_attention_decode has no gradient, forward-mode ones included");
   TORCH_CHECK(q.is_cuda() && q.dim() == 4 && k.dim() == 4 && v.dim() == 4, "q, k and v must be 4-dimensional GPU tensors");
   const int64_t B = q.size(0), Sq = q.size(1), NH = q.size(2), D = q.size(3), S = k.size(1), NKV = k.size(2);
   check_heads(NH, NKV, D);

@@ -32,7 +32,7 @@ from typing import Optional
 import torch
 import torch.nn as nn
 
-from . import require_hip
+from . import refuse_tangents, require_hip
 
 MAX_DISTANCE = 512
 MAX_BUCKETS = 256
@@ -134,7 +134,8 @@ def fused_relative_attention(qkv: torch.Tensor, nh: int, table: torch.Tensor, bu
     """qkv [B, S, (nh + 2 nkv) * D] (all query heads, then key heads, then value
     heads) -> [B, S, nh * D]. ``nkv`` key/value heads (nh if not given) are each
     shared by nh / nkv neighbouring query heads. ``mask8``: [B, S] u8 or bool,
-    1 = attend. ``scale`` defaults to D ** -0.5."""
+    1 = attend. ``scale`` defaults to D ** -0.5. On a GPU there are first
+    derivatives backward alone: forward-mode ones are refused."""
     nkv = nh if nkv is None else nkv
     if qkv.dim() != 3 or nh < 1 or nkv < 1 or nh % nkv or qkv.shape[2] < 1 or qkv.shape[2] % (nh + 2 * nkv):
         raise ValueError(f"qkv must be [B, S, (nh + 2 nkv) * D] with nh a multiple of nkv; got "
@@ -180,6 +181,7 @@ def relative_attention_decode(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     if q.is_cuda:
         _check_gpu(q, D)
         return require_hip().rel_attn_token(q, k, v, table.contiguous(), buckets.contiguous(), lengths.contiguous(), scale)
+    refuse_tangents("relative_attention_decode", q, k, v, table)
     S, NKV = k.shape[1:3]
     up = torch.promote_types(q.dtype, torch.float32)
     n = lengths.long().clamp(0, S)

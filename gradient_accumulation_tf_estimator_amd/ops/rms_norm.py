@@ -21,7 +21,7 @@ from typing import Optional, Tuple
 import torch
 import torch.nn as nn
 
-from . import require_hip
+from . import refuse_tangents, require_hip
 
 FP8_MAX = 448.0  # the largest finite e4m3 value
 GROUPS = (0, 32, 64, 128)
@@ -67,7 +67,7 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch
     share a scale (0: the whole row, groups = 1); a group of zeros has scale 1,
     others at least 2^-126.
     For serving: nothing here has a gradient, so inputs that need one are
-    refused while gradients are recorded."""
+    refused while gradients are recorded, and those with a tangent at all times."""
     _check(x, weight, residual)
     if eps < 0:
         raise ValueError(f"eps must not be negative, got {eps}")
@@ -79,6 +79,7 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch
         raise RuntimeError("rms_norm_fp8 has no gradient: call it under torch.no_grad()")
     if x.is_cuda:
         return tuple(require_hip().rms_norm_fp8(x, residual, weight, eps, group))
+    refuse_tangents("rms_norm_fp8", x, weight, residual)
     groups = x.shape[-1] // group if group else 1
     y, h = _plain(x, weight, residual, eps)
     y = y.reshape(*x.shape[:-1], groups, x.shape[-1] // groups)

@@ -105,5 +105,5 @@ def _plain_clip(got, dst, clip_norm):
     _check_apart(got, dst)
     dst = dst or [torch.empty_like(t) for t in got]
     for d, t in zip(dst, got):
-        d.copy_(t.float() * coef)
+        d.copy_(t.detach().float() * coef)  # detached: no_grad leaves tangents on
     return norm.float(), dst

@@ -1,10 +1,12 @@
-"""Forward-mode derivatives of the norm and relative-attention operators: right where there is a plain form, refused where they would be lost
+"""Forward-mode derivatives of the norm, clipping and relative-attention
+operators: right where there is a plain form, refused where they would be lost
 without a word."""
 
 import pytest
 import torch
 import torch.autograd.forward_ad as fw
 
+from gradient_accumulation_tf_estimator_amd import clip_by_global_norm, global_norm
 from gradient_accumulation_tf_estimator_amd.ops.relative_attention import (
     fused_relative_attention,
     relative_attention_decode,
@@ -30,6 +32,16 @@ def test_decode_refuses_tangents():
             with torch.no_grad(), pytest.raises(RuntimeError, match="no gradient"):
                 relative_attention_decode(*args[:i], fw.make_dual(x, x), *args[i + 1:], m, n)
         relative_attention_decode(*args, m, n)
+
+
+def test_clipped_results_have_no_tangent():
+    """Nor a gradient: the factor's own derivative is in neither."""
+    x = torch.randn(2, 64)
+    with fw.dual_level():
+        dual = fw.make_dual(x, torch.ones_like(x))
+        out, norm = clip_by_global_norm([dual], 1.0)
+        for t in (out[0], norm, global_norm([dual])):
+            assert fw.unpack_dual(t).tangent is None
 
 
 def test_plain_forms_against_differences():
@@ -70,4 +82,6 @@ def test_kernels_refuse_tangents():
                 add_rms_norm(*args)
             with pytest.raises(RuntimeError, match="no gradient"):
                 rms_norm_fp8(*args)
+        out, norm = clip_by_global_norm([fw.make_dual(x, x)], 1.0)
+        assert fw.unpack_dual(out[0]).tangent is None and fw.unpack_dual(norm).tangent is None
         fused_relative_attention(qkv, 2, table, m)  # others are taken inside the level too

@@ -105,6 +105,8 @@ def _bias(table, buckets, rows, cols):
 
 def _softmax(s, keep):
     """softmax over the last axis of what ``keep`` allows; zeros where it allows nothing."""
+    if s.shape[-1] == 0:  # no keys at all
+        return s
     s = s.masked_fill(~keep, -math.inf)
     top = s.detach().amax(-1, keepdim=True)
     p = torch.exp(s - torch.where(torch.isinf(top) & (top < 0), 0.0, top))
@@ -191,8 +193,6 @@ def relative_attention_decode(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     rows = n[:, None] - Sq + torch.arange(Sq)[None]
     keep = (keys[None, None] <= rows[:, :, None])[:, None]
     s = torch.matmul(q.to(up).transpose(1, 2), kk.transpose(2, 3)) * scale + _bias(table.to(up), buckets, rows, keys)
-    if S == 0:
-        return torch.zeros_like(q)
     return torch.matmul(_softmax(s, keep), vv).transpose(1, 2).to(q.dtype)
 
 

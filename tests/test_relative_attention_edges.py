@@ -1,4 +1,7 @@
-"""Relative-bias attention on the CPU without rows: as the kernels take it."""
+"""Relative-bias attention at the ends of its ranges: no rows, no distance to
+speak of, more new tokens than the cache holds, the smallest and largest scales."""
+
+import math
 
 import pytest
 import torch
@@ -28,3 +31,48 @@ def test_empty_caches(B, Sq, S):
     k = torch.zeros(B, S, 2, 8)
     out = relative_attention_decode(torch.randn(B, Sq, 4, 8), k, k, torch.randn(32, 4), m, torch.ones(B, dtype=torch.int32))
     assert out.shape == (B, Sq, 4, 8) and (out == 0).all()
+
+
+def maps(far, buckets):
+    return (torch.arange(2 * far + 1) % buckets).to(torch.int32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("far,buckets", [(1, 1), (1, 3), (2, 4), (512, 1), (512, 256), (37, 5)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_any_map(far, buckets, causal, D):
+    """Short and long distances, one bucket and many, in no order of theirs: against 64 bits, with the CPU's formulas."""
+    torch.manual_seed(far)
+    B, S, NH = 2, 150, 2
+    m = maps(far, buckets)
+    qkv, table, dout = torch.randn(B, S, 3 * NH * D).bfloat16(), torch.randn(buckets, NH).bfloat16(), torch.randn(B, S, NH * D).bfloat16()
+
+    def run(qkv, table, m, dout):
+        a, t = qkv.detach().requires_grad_(), table.detach().requires_grad_()
+        out = fused_relative_attention(a, NH, t, m, causal=causal)
+        return [out.detach(), *torch.autograd.grad(out, (a, t), dout)]
+
+    want = run(qkv.double(), table.double(), m, dout.double())
+    got = run(qkv.cuda(), table.cuda(), m.cuda(), dout.cuda())
+    # out: P and the result rounded to bf16; the gradients: D's, P's, dS's and the result's roundings, 2^-8 each of parts
+    # that are at most some four times the result's own size (norms over all elements). One bucket's gradient is zero:
+    # a row's dS sums to nothing; what is left is what D is off by, a rounding of out for each row.
+    zero = 2.0**-8 * float(dout.double().norm()) if buckets == 1 else 0.0
+    for g, w, roundings, more in zip(got, want, (2, 8, 16), (0.0, 0.0, zero)):
+        assert float((g.cpu().double() - w).norm()) <= roundings * 2.0**-8 * float(w.norm()) + more + 1e-30
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Sq,S", [(5, 3), (40, 7), (3, 1)])
+def test_more_new_tokens_than_the_cache_holds(Sq, S):
+    torch.manual_seed(Sq)
+    m, table = relative_position_buckets(32, 128, False), torch.randn(32, 4).bfloat16()
+    q, k, v = torch.randn(3, Sq, 4, 64).bfloat16(), torch.randn(3, S, 2, 64).bfloat16(), torch.randn(3, S, 2, 64).bfloat16()
+    n = torch.tensor([S, 1, 0], dtype=torch.int32)
+    want = relative_attention_decode(q.double(), k.double(), v.double(), table.double(), m, n)
+    got = relative_attention_decode(q.cuda(), k.cuda(), v.cuda(), table.cuda(), m.cuda(), n.cuda()).cpu().double()
+    # P and the result rounded; sums of at most S terms
+    most = float(v.double().abs().max())
+    assert ((got - want).abs() <= 2 * 2.0**-8 * most + 2.0**-8 * want.abs()).all()
+    assert (got[2] == 0).all() and (got[:, :Sq - S] == 0).all()

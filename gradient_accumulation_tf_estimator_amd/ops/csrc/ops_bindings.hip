@@ -3,7 +3,6 @@
 // current stream of the operands' device.
 
 #include <algorithm>
-#include <cmath>
 #include <cstdint>
 #include <vector>
 
@@ -321,6 +320,12 @@ void check_heads(int64_t NH, int64_t NKV, int64_t D) {
   TORCH_CHECK(NH >= 1 && NKV >= 1 && NH % NKV == 0, "query heads must be a multiple of key/value heads");
 }
 
+// The kernels hold scale and bias / scale in 32 bits; table values are below
+// 2^29, and beyond these bounds one of the two would be zero or infinite.
+void check_scale(double scale) {
+  TORCH_CHECK_VALUE(scale >= 0x1p-96 && scale <= 0x1p96, "scale must be within 2^-96 .. 2^96 on a GPU, got ", scale);
+}
+
 RelArgs rel_args(const at::Tensor& qkv, int64_t NH, int64_t NKV, const at::Tensor& table, const at::Tensor& map,
                  const MaybeTensor& mask, bool causal, double scale) {
   TORCH_CHECK(qkv.is_cuda() && qkv.scalar_type() == at::kBFloat16 && qkv.dim() == 3 && qkv.is_contiguous() &&
@@ -329,7 +334,7 @@ RelArgs rel_args(const at::Tensor& qkv, int64_t NH, int64_t NKV, const at::Tenso
   const int64_t B = qkv.size(0), S = qkv.size(1), D = qkv.size(2) / (NH + 2 * NKV);
   check_heads(NH, NKV, D);
   check_bias(table, map, qkv, NH);
-  TORCH_CHECK(scale > 0 && std::isfinite(scale), "scale must be positive and finite");
+  check_scale(scale);
   // a launch has fewer than 2^32 threads, 512 for each 128 rows of a head; a chunk of 64 rows is addressed by 32 bits from its start
   TORCH_CHECK(qkv.size(2) <= (1 << 23), "too many heads");
   TORCH_CHECK(S < (1ll << 24) && B * NH * (S / 128 + 1) < (1ll << 22), "too many rows");
@@ -473,7 +478,7 @@ at::Tensor rel_attn_token(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor t
   check_bias(table, map, q, NH);
   TORCH_CHECK(lengths.device() == q.device() && lengths.scalar_type() == at::kInt && lengths.is_contiguous() &&
               lengths.dim() == 1 && lengths.numel() == B, "lengths must be an int32 [B] tensor on the same GPU");
-  TORCH_CHECK(scale > 0 && std::isfinite(scale), "scale must be positive and finite");
+  check_scale(scale);
   TORCH_CHECK(NH / NKV <= 32, "at most 32 query heads a key/value head");
   // fewer than 2^32 threads here too
   TORCH_CHECK(S < (1ll << 31) - 64 && B * NH * Sq < (1ll << 22), "too many rows");

@@ -136,8 +136,9 @@ def fused_relative_attention(qkv: torch.Tensor, nh: int, table: torch.Tensor, bu
     """qkv [B, S, (nh + 2 nkv) * D] (all query heads, then key heads, then value
     heads) -> [B, S, nh * D]. ``nkv`` key/value heads (nh if not given) are each
     shared by nh / nkv neighbouring query heads. ``mask8``: [B, S] u8 or bool,
-    1 = attend. ``scale`` defaults to D ** -0.5. On a GPU there are first
-    derivatives backward alone: forward-mode ones are refused."""
+    1 = attend. ``scale`` defaults to D ** -0.5; the kernels take 2^-96 to
+    2^96. On a GPU there are first derivatives backward alone: forward-mode
+    ones are refused."""
     nkv = nh if nkv is None else nkv
     if qkv.dim() != 3 or nh < 1 or nkv < 1 or nh % nkv or qkv.shape[2] < 1 or qkv.shape[2] % (nh + 2 * nkv):
         raise ValueError(f"qkv must be [B, S, (nh + 2 nkv) * D] with nh a multiple of nkv; got "

@@ -76,3 +76,36 @@ def test_more_new_tokens_than_the_cache_holds(Sq, S):
     most = float(v.double().abs().max())
     assert ((got - want).abs() <= 2 * 2.0**-8 * most + 2.0**-8 * want.abs()).all()
     assert (got[2] == 0).all() and (got[:, :Sq - S] == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", [1e-300, 1e-50, 1e-38, 2.0**-97, 2.0**97, 1e39, 1e300])
+def test_scales_beyond_32_bits_are_refused(scale):
+    """In 32 bits they are zero or infinite, or a bias divided by them is."""
+    m, table = relative_position_buckets().cuda(), torch.ones(32, 2, device="cuda").bfloat16()
+    qkv = torch.ones(1, 5, 6 * 64, device="cuda").bfloat16()
+    with pytest.raises(ValueError, match="scale"):
+        fused_relative_attention(qkv, 2, table, m, scale=scale)
+    k, n = torch.ones(1, 5, 2, 64, device="cuda").bfloat16(), torch.ones(1, dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError, match="scale"):
+        relative_attention_decode(k[:, :1], k, k, table, m, n, scale=scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bias", [1.0, -3.0, 2.0**28, -(2.0**28)])
+def test_the_smallest_scale_leaves_the_bias(bias):
+    """Scores that vanish beside a bias that all keys share: the values' mean, and dv is dout's."""
+    torch.manual_seed(1)
+    S = 100
+    m, table = relative_position_buckets().cuda(), torch.full((32, 1), bias, device="cuda").bfloat16()
+    qkv, dout = torch.randn(1, S, 3 * 64).bfloat16(), torch.randn(1, S, 64).bfloat16()
+    a = qkv.cuda().requires_grad_()
+    out = fused_relative_attention(a, 1, table, m, scale=2.0**-96)
+    dv = torch.autograd.grad(out, a, dout.cuda())[0][..., 128:].cpu().double()
+    v, g = qkv[..., 128:].double(), dout.double()
+    # P, dO where the sum stands apart, and the result, a rounding each of the values' absolute sums
+    for got, x in ((out.detach().cpu().double(), v), (dv, g)):
+        assert ((got - x.mean(1, keepdim=True)).abs() <= 3 * 2.0**-8 * x.abs().mean(1, keepdim=True)).all()
+    q, n = qkv.cuda().view(1, S, 3, 64), torch.full((1,), S, dtype=torch.int32, device="cuda")
+    got = relative_attention_decode(q[:, -1:, :1], q[:, :, 1:2], q[:, :, 2:], table, m, n, scale=2.0**-96).cpu().double()
+    assert ((got[0, 0] - v.mean(1)).abs() <= 3 * 2.0**-8 * v.abs().mean(1)).all()

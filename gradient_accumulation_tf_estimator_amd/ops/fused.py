@@ -171,6 +171,9 @@ def flush_pending_wgrads() -> None:
 
 def set_wgrad_overlap(enabled: bool) -> None:
     global _WGRAD_OVERLAP
+    if _WGRAD_OVERLAP and not enabled and _wgrad_stream is not None:
+        # the engine joins the side stream only while the switch is on
+        torch.cuda.current_stream().wait_stream(_wgrad_stream)
     _WGRAD_OVERLAP = bool(enabled)
 
 

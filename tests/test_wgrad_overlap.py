@@ -211,3 +211,27 @@ def test_encoder_with_the_side_stream_and_without(norm, monkeypatch):
         torch.cuda.synchronize()
         near(model, engine, want[step])
         torch.randn(1000, device="cuda").sum().item()
+
+
+def test_switching_it_off_waits_for_what_is_running(monkeypatch):
+    """The engine joins the side stream only while the switch is on."""
+    waited = []
+
+    class Main:
+        def wait_stream(self, other):
+            waited.append(other)
+
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda *a: Main())
+    monkeypatch.setattr(fused, "_wgrad_stream", None)
+    monkeypatch.setattr(fused, "_WGRAD_OVERLAP", False)
+    fused.set_wgrad_overlap(True)
+    fused.set_wgrad_overlap(False)  # nothing ran there
+    assert not waited
+    fused.set_wgrad_overlap(True)
+    monkeypatch.setattr(fused, "_wgrad_stream", "side")
+    fused.set_wgrad_overlap(True)
+    assert not waited
+    fused.set_wgrad_overlap(False)
+    assert waited == ["side"]
+    fused.set_wgrad_overlap(False)
+    assert waited == ["side"]

@@ -8,8 +8,8 @@
 // factor needs them all first. A tensor is cut into chunks, one block each; the
 // tensors' addresses travel by value with the launch (up to 128 a launch), so
 // nothing is copied to the device, nothing is kept between calls, and a
-// captured graph holds all that it needs. 335M fp32 elements in 391 tensors: 803 us
-// for 4.0 GB (5.0 TB/s), 253 us of it the norm's pass; 28.7M bf16: 34 us (13 the
+// captured graph holds all that it needs. 335M fp32 elements in 391 tensors: 802 us
+// for 4.0 GB (5.0 TB/s), 251 us of it the norm's pass; 28.7M bf16: 34 us (13 the
 // norm, 4 its end, 19 the scaling).
 //
 // Squares are taken and summed in 64 bits: a bf16 or fp32 gradient's square

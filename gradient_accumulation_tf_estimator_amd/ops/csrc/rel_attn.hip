@@ -27,9 +27,10 @@
 // Rounded to bf16: P and dS before the second product (a relative 2^-9 of each,
 // which the matrix instruction's operands force), and the outputs.
 //
-// Times at each kernel are medians on one MI355X of two workloads: "padded",
-// 16x512 with lengths of all sizes, 12 heads, D 64; "long", 2x4093 causal, 16
-// heads over 4, D 128. The forward and both backward kernels are bound by the
+// Times at each kernel are medians of 200 passes under the profiler on one
+// MI355X of two workloads: "padded", 16x512 with lengths of all sizes, 12 heads,
+// D 64; "long", 2x4093 causal, 16 heads over 4, D 128. (The first 20 passes
+// of the long case took 173, 267 and 341 us there.) The forward and both backward kernels are bound by the
 // vector unit beside the matrix unit: a 32x32 tile takes 8 matrix instructions at
 // D 64 in the forward and some 90 vector ones (16 exponentials at a quarter of
 // the rate), and two waves of a SIMD overlap them little (16 matrix instructions
@@ -64,7 +65,8 @@ constexpr int TILE = GA_REL_TILE;  // rows of a workgroup: four waves of 32
 // LDS serves 256 bytes at a time: sixteen neighbouring rows' pieces at one
 // column (row reads), or 64 bytes of each of four neighbouring rows (the
 // transposing reads); the function sends both to 256 bytes of different banks
-// (a row of D = 64 is half of them, and which half is its lowest bit).
+// (a row of D = 64 is half of them, and which half is its lowest bit). So the
+// tiles' reads do not conflict; those of the bias do, see bias_tile.
 template <int D>
 __device__ __forceinline__ int piece(int row, int p) {
   const int f = D == 64 ? ((row >> 1) & 1) << 2 | ((row >> 2) & 3) : (row & 3) << 2 | ((row >> 2) & 3);
@@ -124,8 +126,9 @@ __device__ __forceinline__ b8 pack(const f16& c, int ks) {
 // waits for a load: the next chunk arrives while this one is computed. The
 // tile's order is made by the addresses that the lanes read. Issued by inline
 // assembly, because behind the builtin the compiler waits for the data before
-// any LDS read that follows; nothing else in these kernels uses m0, and the
-// instruction has no register result. After `wait`, `clear` zeroes the rows
+// any LDS read that follows; the instruction has no register result. m0 is
+// reserved, so the compiler takes no clobber of it: in the code that it makes of
+// these kernels no other instruction names m0. After `wait`, `clear` zeroes the rows
 // that must not count (masked keys, rows past the end): what stands there, NaN
 // too, cannot reach a result. Ordinary loads of the loop are issued before the
 // chunk's and used after `wait`, or their own wait would be for the chunk too.
@@ -262,6 +265,11 @@ struct Bias {
 
 // C's initial value for rows u0 + crow(r) against column w: the bias of the
 // offset row - column. `low`, `high`: the values beyond the largest distance.
+// The four copies lie bias_len floats apart, 12 modulo the 64 banks at distances
+// 64, 128, 256 and 512: the sixteen lanes of a read touch 13 different places of
+// 16 bytes instead of 16, so it takes twice its time. That is what the counters
+// show as conflicts: 27, 19 and 17 % of the LDS cycles of the three kernels on
+// "padded", 5, 4 and 2 % on "long".
 __device__ __forceinline__ f16 bias_tile(const float* bias, int far, int row0, int col0, int lane, float low, float high) {
   f16 c;
   if (row0 + 31 - col0 <= -far || row0 - (col0 + 31) >= far) {
@@ -396,7 +404,7 @@ __device__ __forceinline__ void save_lse(float* lse, long long rows, float m, fl
 }
 
 // ---------------- forward: a wave owns 32 queries, chunks of 64 keys ----------------
-// padded 24 us (matrix unit 22 % busy), long 163 us (47 %, 841 TFLOP/s)
+// padded 23 us (matrix unit 22 % busy), long 160 us (47 %, 859 TFLOP/s)
 template <int D>
 __global__ __launch_bounds__(256, 2) void k_rel_fwd(RelArgs a, int tiles) {
   extern __shared__ __align__(16) char smem[];  // the tiles lie in the first 64 KB, which m0 reaches
@@ -598,7 +606,7 @@ __device__ __forceinline__ void diagonals_32(const f16& c, float* d, bool ib) {
 }
 
 // ---------------- backward 1: dQ, D and the offsets' sums of dS ----------------
-// padded 38 us (matrix unit 19 % busy), long 243 us (43 %, 848 TFLOP/s)
+// padded 36 us (matrix unit 19 % busy), long 240 us (43 %, 857 TFLOP/s)
 template <int D>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_rel_bwd_q(RelArgs a, int tiles) {
   extern __shared__ __align__(16) char smem[];  // the tiles lie in the first 64 KB, which m0 reaches
@@ -901,7 +909,7 @@ __device__ void sum_table(const RelArgs& a, int h, char* smem) {
 // 128. V is kept in LDS there, by eight waves that share a chunk instead of four:
 // two waves a SIMD (long: 480 us with V in registers, 340 so, when that step was
 // taken; padded: 45 us with V in registers, 61 in LDS with four waves, 85 with
-// eight). padded 43 us (matrix unit 22 % busy), long 297 us (43 %, 925 TFLOP/s),
+// eight). padded 42 us (matrix unit 22 % busy), long 294 us (43 %, 934 TFLOP/s),
 // the table's sums among them.
 template <int D>
 constexpr int kv_waves() { return D == 64 ? 4 : 8; }
@@ -1095,8 +1103,8 @@ __global__ __launch_bounds__(256) void k_rel_dkv(RelArgs a, long long n) {
 // instead of 7.5); a wave takes 32 keys at a time, K straight into A fragments, V
 // through its own LDS tile. The waves' (maximum, sum, output) are joined in LDS,
 // the workgroups' by k_rel_join. Bound by the cache's bytes: 16 sequences of up to
-// 16384 tokens, 16 heads over 4, D 128: 90 us with the join, 4.5 TB/s of
-// the 4.9 that a copy reaches.
+// 16384 tokens, 16 heads over 4, D 128: 88 to 91 us with the join, 4.4 to 4.6 TB/s
+// of the 4.9 that a copy reaches.
 constexpr int TOKEN_WAVES = 8;
 template <int D>
 __global__ __launch_bounds__(512) void k_rel_token(RelTokenArgs a, int row_tiles) {
@@ -1261,7 +1269,7 @@ __global__ __launch_bounds__(512) void k_rel_token(RelTokenArgs a, int row_tiles
   }
 }
 
-// joins the workgroups' parts of one output row, in order (4.8 us at 256 rows of 8 parts, D 128)
+// joins the workgroups' parts of one output row, in order (4.9 us at 256 rows of 8 parts, D 128)
 template <int D>
 __global__ __launch_bounds__(D) void k_rel_join(RelTokenArgs a, int row_tiles) {
   const int group = a.NH / a.NKV, rows = group * a.Sq;

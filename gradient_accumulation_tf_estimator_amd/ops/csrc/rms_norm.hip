@@ -12,9 +12,10 @@
 // exchange, no barrier) and one 256-thread block a row above (one barrier a
 // statistic). The next row's loads are issued before this row's reduction.
 // 32768 rows of 4096 bf16: forward with a residual 182 us (1.07 GB, 5.9 TB/s, the
-// last level cache helping), backward 241 us (4.5 TB/s) and 7 us for dw's sum; a
-// large copy reaches 4.9. 16384 rows to 8 bits: 92 us (472 MB, 5.1 TB/s). 1024 rows
-// of 512: 3.4, 3.9 and 2.6 us, which is the latency of a launch.
+// last level cache helping), backward 235 us (1.07 GB, 4.6 TB/s) and 7 us for dw's
+// sum; a large copy reaches 4.9. 16384 rows to 8 bits: 93 us a call (472 MB, 5.1
+// TB/s, that cache helping here too). 1024 rows of 512: 3.3, 3.9 and 2.5 us, which
+// is the latency of a launch.
 //
 // Sums, statistics and the norm itself are held in 32 bits. The forward norms
 // the sum before it is rounded to the stream's type, so y carries one rounding;
